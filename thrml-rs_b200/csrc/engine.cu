@@ -174,32 +174,6 @@ struct thrml_moments {
 // ---------------------------------------------------------------------------------------------------------
 // Host helpers.
 // ---------------------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void* sym = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(sym);
-    }
-    return fn;
-}
-// 2-D K-major operand: `rows` rows of `k_elems` contiguous elements, row pitch in bytes; box = 128 bytes of K x box_rows,
-// 128-byte swizzle, out-of-range elements read as zero.
-static int32_t make_operand_map(CUtensorMap* map, void* base, bool is_u8, int64_t k_elems, int64_t rows, int64_t pitch_bytes, int box_rows) {
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (!fn) return fail(THRML_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k_elems), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
-    const cuuint32_t box[2] = {static_cast<cuuint32_t>(is_u8 ? 128 : 64), static_cast<cuuint32_t>(box_rows)};
-    const cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, is_u8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(THRML_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string(static_cast<int>(r)));
-    return THRML_OK;
-}
 // Width of a CTA pair's tile for n output columns: the candidate that pads n the least, the wider one on ties.
 static int32_t pair_tile_width(int64_t n) {
     int32_t best = 256;
