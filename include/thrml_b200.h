@@ -507,6 +507,92 @@ int32_t thrml_potts_sample_with_marginals(thrml_potts* p, uint64_t key, int64_t 
 int32_t thrml_potts_marginals_allreduce(thrml_potts* p, thrml_comm* comm);
 int32_t thrml_potts_synchronize(thrml_potts* p);
 
+/* ------------------------------------------------------------------------------------------------
+ * Categorical readout (no counterpart in the reference, whose categorical nodes hold at most 256 categories and whose
+ * logits come from factor tables): a model whose categories are many and whose logits come from a layer of weights.
+ * thrml_linear_i8 turns activations into logits, thrml_adjust_logits applies the rules of a generation step,
+ * thrml_draw_categories draws from them under an RngKey as the categorical samplers do, and thrml_distill_* train the
+ * logits against a teacher.
+ *
+ * These calls work on the caller's DEVICE memory of the context's device and on the caller's stream (`stream` is a
+ * cudaStream_t, NULL = the legacy default stream; thrml_ctx_stream gives the context's own).  They are asynchronous,
+ * allocate nothing, keep nothing between calls and can be captured into a CUDA graph; two threads may use one context for
+ * them.  Element types are THRML_F32, THRML_BF16, THRML_F16 (indices: THRML_I32, THRML_I64); a pitch is the distance of two
+ * rows in elements, at least the row's length; the elements of a row are contiguous.  Pointers are aligned to their element.
+ * Inputs and outputs do not overlap except where a call says so.  A call with no rows does nothing.
+ * ---------------------------------------------------------------------------------------------- */
+#define THRML_F32 0
+#define THRML_BF16 1
+#define THRML_F16 2
+#define THRML_I32 3
+#define THRML_I64 4
+/* 8-bit rows: scale[r] = max_k |x[r][k]| / 127 (f32), q[r][k] = x[r][k] / scale[r] rounded to nearest even and held within
+ * +-127; elements of q from cols up to q_pitch are not written.  A row of zeros has scale 0 and zeros; a row with an infinity or
+ * a NaN has that (or NaN) as its scale and zeros, so that what is made of it is NaN. */
+int32_t thrml_quantize_rows_i8(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
+                               float* scale);
+/* out[i][j] = (sum_k a[i][k] w[j][k]) * a_scale[i] * w_scale[j] + bias[j] (bias f32, nullable): 8-bit integers, one scale for
+ * each token (row of a) and channel (row of w), the sum exact in 32-bit integers (k at most 131071), the rest in f32, rounded
+ * once to out_type.  a and w start on 16-byte boundaries and their pitches are multiples of 16. */
+int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* w,
+                        int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch);
+/* Both: x is quantised into q (16-byte boundary, pitch a multiple of 16) and scale, the caller's workspaces, then multiplied. */
+int32_t thrml_linear_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
+                        float* scale, const int8_t* w, int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch);
+/* The rules of one generation step on logits[rows][cols], in this order (all in f32, rounded once to the logits' type):
+ *   history   row r has seen the tokens history[history_ptr[r] .. history_ptr[r+1]) (history_type THRML_I32 or THRML_I64), the first
+ *             n_prompt[r] of them as its prompt (nullable = none of them); tokens outside [0, cols) are padding;
+ *   penalties a category seen at all: x > 0 ? x / repetition[r] : x * repetition[r]; then, for a category seen o > 0 times behind
+ *             the prompt, x - frequency[r] * o - presence[r] (each nullable = off; repetition > 0);
+ *   biases    x + bias_values[e] for the entries e in [bias_ptr[r], bias_ptr[r+1]) whose bias_ids[e] is the category (entries that
+ *             repeat a category add up, next to each other in their order; ids outside [0, cols) are padding);
+ *   mask      -infinity where bit k & 31 of word k >> 5 of the row's mask is 0.  mask[n_masks][mask_pitch] words; the row's
+ *             mask is mask_rows[r], none when that lies outside [0, n_masks); mask_rows NULL: mask r for row r.
+ * `out` may be `logits` itself (same pitch).  rules->history, bias_ids and mask are each nullable = off. */
+typedef struct thrml_logit_rules {
+    const void* history;
+    const int64_t* history_ptr; /* [rows + 1], ascending */
+    const int32_t* n_prompt;    /* [rows] */
+    const float* repetition;    /* [rows] */
+    const float* frequency;     /* [rows] */
+    const float* presence;      /* [rows] */
+    const int32_t* bias_ids;
+    const float* bias_values;
+    const int64_t* bias_ptr; /* [rows + 1], ascending */
+    const uint32_t* mask;
+    const int32_t* mask_rows; /* [rows] */
+    int64_t n_masks, mask_pitch;
+    int32_t history_type;
+} thrml_logit_rules;
+int32_t thrml_adjust_logits(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, void* out, int64_t out_pitch,
+                            const thrml_logit_rules* rules);
+/* One category per row: out[r] = argmax_k beta[r] * logits[r][k] - log(-log(u_rk)), ties to the lowest k; beta NULL = 1.  A row with
+ * beta = infinity takes the largest logit (no noise).  Categories at -infinity or NaN are never drawn; a row that has no other,
+ * or whose beta is negative or NaN, gets -1.  The uniforms: noise[r][k] in (0, 1) (f32, device; the injected noise of a
+ * parity run), or with noise NULL the 23-bit uniform of word k & 3 of Philox4x32-10(counter (row_offset + r, 0, k >> 2, 'DRAW'), key),
+ * so that results do not depend on how rows are sharded (row_offset + rows <= 2^32).  Scores that lie near the largest
+ * are compared in f64. */
+int32_t thrml_draw_categories(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, const float* beta, uint64_t key,
+                              int64_t row_offset, const float* noise, int64_t noise_pitch, int64_t* out);
+/* Distillation from a teacher's top logits.  Row r lists categories ids[r][0 .. top) (top <= 1024; THRML_I32 or THRML_I64) with the teacher's logits;
+ * entries whose id lies outside [0, cols) or whose logit is -infinity are not listed, a category listed twice counts twice.
+ *   p = softmax over the listed of beta * teacher,  q = softmax over all categories of beta * logits,
+ *   loss[r] = sum_j p_j (log p_j - log q_id(j)),    grad[r][k] = weight[r] * beta * (q_k - p_k)   (p_k summed over entries)
+ * = weight[r] times the derivative of loss[r] by logits[r][k]; weight NULL = 1; beta > 0, finite.  A row of weight 0 (padding) is not
+ * read: its loss and gradient are 0.  A row that lists nothing likewise.  A row of logits that are all -infinity has q = 0 and
+ * loss = infinity.  thrml_distill_loss also writes lse[r] = log sum_k exp(beta * logits[r][k]) (0 for rows not read), which
+ * thrml_distill_grad takes back; thrml_distill_step gives loss and gradient with the weights known beforehand, reading the
+ * logits once.  grad has the logits' type; it may be `logits` itself (same pitch). */
+int32_t thrml_distill_loss(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, int64_t top, const void* ids,
+                           int32_t ids_type, int64_t ids_pitch, const void* teacher, int32_t teacher_type, int64_t teacher_pitch, float beta, const float* weight,
+                           float* loss, float* lse);
+int32_t thrml_distill_grad(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, int64_t top, const void* ids,
+                           int32_t ids_type, int64_t ids_pitch, const void* teacher, int32_t teacher_type, int64_t teacher_pitch, float beta, const float* weight,
+                           const float* lse, void* grad, int64_t grad_pitch);
+int32_t thrml_distill_step(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, int64_t top, const void* ids,
+                           int32_t ids_type, int64_t ids_pitch, const void* teacher, int32_t teacher_type, int64_t teacher_pitch, float beta, const float* weight,
+                           float* loss, void* grad, int64_t grad_pitch);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,5 +12,7 @@ from .api import (Block, BlockGibbsSpec, BlockSamplingProgram, BlockSpec, Catego
                   SoftmaxConditional, SpinEBMFactor, SpinGibbsConditional, SquareDiscreteEBMFactor, StateObserver, coloring_to_blocks, estimate_kl_grad, estimate_moments,
                   bipartite_coloring, generate_chain_graph, generate_lattice_graph, greedy_coloring, hinton_init, make_nearest_neighbor_lattice, run_blocks, sample_blocks,
                   sample_states, sample_with_observation)
+from .readout import (adjust_logits, align_rows_int8, distill_grad, distill_loss, distill_step, draw_categories, int8_linear, int8_matmul,  # noqa: F401
+                      quantize_rows)
 
 lib()  # fail at import time when the compiled library is absent: there is no other compute path

@@ -127,11 +127,25 @@ _SIGNATURES = {
     "thrml_potts_sample_with_marginals": (C.c_int32, [_P, C.c_uint64, C.c_int64, C.c_int64, C.c_int64]),
     "thrml_potts_marginals_allreduce": (C.c_int32, [_P, _P]),
     "thrml_sample_with_observation": (C.c_int32, [_P, C.c_uint64, C.c_int64, C.c_int64, C.c_int64, _P, _P, C.c_int32, _P, _P]),
+    "thrml_quantize_rows_i8": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int64, _P]),
+    "thrml_matmul_i8": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int64]),
+    "thrml_linear_i8": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int64, _P, _P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int64]),
+    "thrml_adjust_logits": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int64, _P]),
+    "thrml_draw_categories": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_uint64, C.c_int64, _P, C.c_int64, _P]),
+    "thrml_distill_loss": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P]),
+    "thrml_distill_grad": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P, C.c_int64]),
+    "thrml_distill_step": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P, C.c_int64]),
 }
 
 
 class Noise(C.Structure):
     _fields_ = [("u", C.c_void_p), ("len", C.c_int64)]
+
+
+class LogitRules(C.Structure):
+    """thrml_logit_rules."""
+    _fields_ = [(name, C.c_void_p) for name in ("history", "history_ptr", "n_prompt", "repetition", "frequency", "presence", "bias_ids", "bias_values", "bias_ptr",
+                                                "mask", "mask_rows")] + [("n_masks", C.c_int64), ("mask_pitch", C.c_int64), ("history_type", C.c_int32)]
 
 
 class ThrmlError(ValueError):

@@ -11,8 +11,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_obj")
 OUT = os.path.join(HERE, "libthrml_b200.so")
-SOURCES = ["engine.cu", "lattice.cu", "potts.cu", "comm.cu", "compile_device.cu", "builder.cpp"]
-HEADERS = ["tables.h", "ctx.h", "comm.h", "devbuf.h", "dense.cuh", "tensor_core.cuh", "device_math.cuh", "update_kernels.cuh", "observer_kernels.cuh",
+SOURCES = ["engine.cu", "lattice.cu", "potts.cu", "comm.cu", "compile_device.cu", "readout_logits.cu", "readout_matmul.cu", "builder.cpp"]
+HEADERS = ["tables.h", "ctx.h", "comm.h", "devbuf.h", "dense.cuh", "tensor_core.cuh", "readout.cuh", "device_math.cuh", "update_kernels.cuh", "observer_kernels.cuh",
            os.path.join("..", "..", "include", "thrml_b200.h")]
 FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=default"]
 

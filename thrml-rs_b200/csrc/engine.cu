@@ -239,6 +239,9 @@ int32_t thrml_ctx_create(int32_t device_id, thrml_ctx** out) {
     cudaDeviceProp prop;
     CU_TRY(cudaGetDeviceProperties(&prop, device_id));
     ctx->sm_count = prop.multiProcessorCount;
+    CU_TRY(cudaHostAlloc(reinterpret_cast<void**>(&ctx->wait_flag), sizeof(int), cudaHostAllocMapped));
+    *ctx->wait_flag = 0;
+    CU_TRY(cudaHostGetDevicePointer(reinterpret_cast<void**>(&ctx->wait_flag_dev), ctx->wait_flag, 0));
     *out = ctx.release();
     return THRML_OK;
 }
@@ -247,12 +250,13 @@ void thrml_ctx_destroy(thrml_ctx* ctx) {
     cudaSetDevice(ctx->device);
     cudaDeviceSynchronize();
     if (ctx->stream) cudaStreamDestroy(ctx->stream);
+    if (ctx->wait_flag) cudaFreeHost(ctx->wait_flag);
     delete ctx;
 }
 int32_t thrml_ctx_synchronize(thrml_ctx* ctx) {
     if (!ctx) return fail(THRML_ERR_INVALID_ARG, "null context");
     CU_TRY(cudaStreamSynchronize(ctx->stream));
-    return THRML_OK;
+    return ctx->check_waits();
 }
 void* thrml_ctx_stream(thrml_ctx* ctx) { return ctx ? static_cast<void*>(ctx->stream) : nullptr; }
 

@@ -1,0 +1,359 @@
+// The readout's 8-bit product: activations quantised with one scale per token, weights with one scale per channel, the sum
+// of products exact in 32-bit integers on the tensor cores (tcgen05 kind::i8, accumulators in tensor memory).
+#include "readout.cuh"
+#include "tensor_core.cuh"
+
+using namespace thrml;
+using namespace thrml::readout;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------
+// Rows in 8 bits.
+// ---------------------------------------------------------------------------------------------------------
+// The integer nearest to x / scale, halves to even, within +-127: what dividing in f64 and rounding gives.  x * (1 / scale)
+// is within 2^-15 of the quotient, so only a product that close to a half is decided exactly: x - (h * scale) is one
+// rounding, whose sign is right.
+__device__ __forceinline__ int32_t quantise(float x, float scale, float inverse) {
+    const float t = x * inverse;
+    float q = rintf(t);
+    if (fabsf(fabsf(t - q) - 0.5f) < 0x1p-12f) {
+        const float low = floorf(t), half = low + 0.5f;  // the border between low and low + 1
+        const float over = fmaf(-half, scale, x);
+        q = over > 0.0f ? low + 1.0f : over < 0.0f ? low : 2.0f * rintf(half * 0.5f);
+    }
+    return static_cast<int32_t>(fminf(fmaxf(q, -127.0f), 127.0f));
+}
+
+constexpr int QUANT_THREADS = 256;
+
+struct QuantArgs {
+    const void* x;
+    int64_t x_pitch;
+    int8_t* q;
+    int64_t q_pitch;
+    float* scale;
+    int32_t cols;
+};
+
+// One CTA per row: the largest magnitude, then the row once more.
+template <class T>
+__global__ void __launch_bounds__(QUANT_THREADS) k_quantize(const QuantArgs g) {
+    __shared__ uint32_t sh[QUANT_THREADS / 32];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(g.x) + row * g.x_pitch;
+    int8_t* q = g.q + row * g.q_pitch;
+    uint32_t most = 0;  // the bits of |x| order as the magnitudes do, with infinity and then NaN above them
+    for_row<T>(x, g.cols, tid, QUANT_THREADS, [&](int32_t, const float* v, auto cnt) {
+#pragma unroll
+        for (int j = 0; j < decltype(cnt)::value; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    });
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((tid & 31) == 0) sh[tid >> 5] = most;
+    __syncthreads();
+    for (int w = 0; w < QUANT_THREADS / 32; ++w) most = max(most, sh[w]);
+    const float scale = __fdiv_rn(__uint_as_float(most), 127.0f);
+    if (tid == 0) g.scale[row] = scale;
+    const bool zeros = scale == 0.0f || !(scale < INFINITY);
+    const float lift = scale < 0x1p-100f ? 0x1p100f : 1.0f;  // a power of two: exact, and the reciprocal stays finite
+    const float lifted = scale * lift, inverse = 1.0f / lifted;
+    for_row<T>(x, g.cols, tid, QUANT_THREADS, [&](int32_t i, const float* v, auto cnt) {
+        constexpr int N = decltype(cnt)::value;
+#pragma unroll
+        for (int j = 0; j < N; ++j) q[i + j] = static_cast<int8_t>(zeros ? 0 : quantise(v[j] * lift, lifted, inverse));
+    });
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// The product.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int TILE_N = 128;  // channels of a tile = tensor-memory lanes
+constexpr int KB = 128;      // bytes of K per stage: one 128-byte swizzle atom
+constexpr int PROD_THREADS = 192;  // TMA warp, MMA warp, four epilogue warps
+
+struct ProductArgs {
+    int32_t m, n, k_steps;
+    const float* a_scale;
+    const float* w_scale;
+    const float* bias;
+    void* out;
+    int64_t out_pitch;
+    int* err;
+};
+
+template <int BM>
+__host__ __device__ constexpr int prod_stages() { return BM <= 64 ? 4 : 3; }
+template <int BM>
+constexpr size_t prod_smem(int split) {
+    return 1024 + static_cast<size_t>(prod_stages<BM>()) * (TILE_N + BM) * KB + (split > 1 ? sizeof(int32_t) * TILE_N * BM : 0);
+}
+
+// A CTA computes a tile of TILE_N channels x BM tokens: the channels are the tensor memory's lanes, so a warp's stores run along
+// a row of the output, and few tokens still fill the MMA's 128 rows.  The CTAs of a cluster (1, 2, 4 or 8) share a tile:
+// each takes a part of K, hands its 32-bit sums over through distributed shared memory, and finishes a part of the tokens.
+template <int BM, class T>
+__global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const ProductArgs g) {
+    using namespace dense;
+    constexpr int STAGES = prod_stages<BM>();
+    constexpr uint32_t W_BYTES = TILE_N * KB, STAGE_BYTES = W_BYTES + BM * KB;
+    constexpr uint32_t TMEM_COLS = BM < 32 ? 32 : BM;
+    constexpr uint32_t IDESC = make_idesc(2, 1, TILE_N, BM);  // s32 accumulators, signed 8-bit operands
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full;
+    __shared__ uint32_t tmem_base_slot;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t split;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(split));
+    const uint32_t rank = cluster_rank();
+    const int32_t n0 = static_cast<int32_t>(blockIdx.x / split) * TILE_N, m0 = static_cast<int32_t>(blockIdx.y) * BM;
+    const int32_t k_begin = static_cast<int32_t>(static_cast<int64_t>(g.k_steps) * rank / split), k_end = static_cast<int32_t>(static_cast<int64_t>(g.k_steps) * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        mbar_init(&acc_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_base_slot;
+    if (split > 1) cluster_sync_all();  // the sums cross the cluster only after every CTA has started
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            for (int32_t kt = k_begin; kt < k_end; ++kt) {
+                if (!mbar_wait(&empty_bar[stage], phase ^ 1u, g.err, 1)) break;
+                mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
+                const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
+                tma_load_2d(dst, &map_w, &full_bar[stage], kt * KB, n0);
+                tma_load_2d(dst + W_BYTES, &map_a, &full_bar[stage], kt * KB, m0);
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool alive = true;
+            for (int32_t kt = k_begin; kt < k_end; ++kt) {
+                if (!mbar_wait(&full_bar[stage], phase, g.err, 3)) { alive = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t w_addr = smem_u32(smem + stage * STAGE_BYTES);
+                const uint64_t dw = make_smem_desc(w_addr), da = make_smem_desc(w_addr + W_BYTES);
+#pragma unroll
+                for (int ks = 0; ks < KB / 32; ++ks)
+                    umma<1>(tmem, dw + static_cast<uint64_t>(ks * 2), da + static_cast<uint64_t>(ks * 2), IDESC, kt > k_begin || ks ? 1u : 0u);
+                umma_commit(&empty_bar[stage]);
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (alive) umma_commit(&acc_full);
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, ch = quarter * 32 + lane;
+        const int32_t col = n0 + ch;
+        const float w_scale = col < g.n ? g.w_scale[col] : 0.0f, bias = g.bias && col < g.n ? g.bias[col] : 0.0f;
+        T* out = static_cast<T*>(g.out) + col;
+        auto finish = [&](int32_t token, int32_t acc) {
+            if (token < g.m && col < g.n) {
+                const float y = __int2float_rn(acc) * __ldg(g.a_scale + token) * w_scale;
+                out[token * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
+            }
+        };
+        const bool alive = mbar_wait(&acc_full, 0, g.err, 4);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        int32_t* red = reinterpret_cast<int32_t*>(smem + STAGES * STAGE_BYTES);  // [source CTA][token of the share][channel]
+        const int32_t share = BM / static_cast<int32_t>(split);
+        __syncwarp();
+        for (int c = 0; c < BM / 16; ++c) {
+            uint32_t acc[16];
+            tmem_ld16_issue(taddr + c * 16, acc);
+            tmem_ld_wait();
+            if (split == 1) {
+                if (alive)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) finish(m0 + c * 16 + j, static_cast<int32_t>(acc[j]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const uint32_t t = c * 16 + j, owner = t / share;
+                    const uint32_t at = smem_u32(red + (rank * share + (t - owner * share)) * TILE_N + ch);
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(at, owner)), "r"(acc[j]) : "memory");
+                }
+            }
+        }
+    }
+    if (split > 1) {
+        cluster_sync_all();  // every CTA's sums have arrived
+        if (warp >= 2) {
+            const int quarter = warp & 3, ch = quarter * 32 + lane;
+            const int32_t col = n0 + ch, share = BM / static_cast<int32_t>(split);
+            const int32_t* red = reinterpret_cast<const int32_t*>(smem + STAGES * STAGE_BYTES);
+            if (col < g.n) {
+                const float w_scale = g.w_scale[col], bias = g.bias ? g.bias[col] : 0.0f;
+                T* out = static_cast<T*>(g.out) + col;
+                for (int32_t t = 0; t < share; ++t) {
+                    const int32_t token = m0 + static_cast<int32_t>(rank) * share + t;
+                    if (token >= g.m) break;
+                    int32_t acc = 0;
+                    for (uint32_t src = 0; src < split; ++src) acc += red[(src * share + t) * TILE_N + ch];
+                    const float y = __int2float_rn(acc) * __ldg(g.a_scale + token) * w_scale;
+                    out[token * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+struct Product {
+    int64_t m, n, k;
+    const int8_t* a;
+    int64_t a_pitch;
+    const float* a_scale;
+    const int8_t* w;
+    int64_t w_pitch;
+    const float* w_scale;
+    const float* bias;
+    void* out;
+    int32_t out_type;
+    int64_t out_pitch;
+};
+
+int32_t check_matrix8(const char* what, const void* p, int64_t k, int64_t pitch) {
+    if (!p) return fail(THRML_ERR_INVALID_ARG, std::string(what) + ": null pointer");
+    if (!aligned_to(p, 16) || pitch % 16) return fail(THRML_ERR_INVALID_ARG, std::string(what) + ": 8-bit rows start on 16-byte boundaries and have a pitch that is a multiple of 16");
+    if (pitch < k) return fail(THRML_ERR_INVALID_ARG, std::string(what) + ": the pitch is smaller than a row");
+    return THRML_OK;
+}
+
+int32_t check_product(const Product& p) {
+    if (p.m < 0 || p.m > (1 << 22) || p.n < 0 || p.n > (1 << 24)) return fail(THRML_ERR_INVALID_ARG, "at most 2^22 tokens and 2^24 channels");
+    if (p.k < 1 || p.k > 131071) return fail(THRML_ERR_INVALID_ARG, "k is not within 1 and 131071, where sums of 8-bit products fit 32 bits");
+    if (!is_float_type(p.out_type)) return fail(THRML_ERR_INVALID_ARG, "out: the element type is not a float type");
+    if (p.m == 0 || p.n == 0) return THRML_OK;
+    if (p.out_pitch < p.n) return fail(THRML_ERR_INVALID_ARG, "out: the pitch is smaller than a row");
+    if (!p.out || !aligned_to(p.out, type_size(p.out_type))) return fail(THRML_ERR_INVALID_ARG, "out: the pointer is null or not aligned to the element");
+    if (!p.a_scale || !p.w_scale) return fail(THRML_ERR_INVALID_ARG, "scales: null pointer");
+    if (int32_t rc = check_matrix8("a", p.a, p.k, p.a_pitch)) return rc;
+    return check_matrix8("w", p.w, p.k, p.w_pitch);
+}
+
+template <int BM, class T>
+int32_t launch_product(thrml_ctx* ctx, cudaStream_t stream, const Product& p, int split) {
+    CUtensorMap map_w, map_a;
+    if (int32_t rc = make_operand_map(&map_w, const_cast<int8_t*>(p.w), true, p.k, p.n, p.w_pitch, TILE_N)) return rc;
+    if (int32_t rc = make_operand_map(&map_a, const_cast<int8_t*>(p.a), true, p.k, p.m, p.a_pitch, BM)) return rc;
+    ProductArgs g{static_cast<int32_t>(p.m), static_cast<int32_t>(p.n), static_cast<int32_t>((p.k + KB - 1) / KB), p.a_scale, p.w_scale, p.bias, p.out, p.out_pitch, ctx->wait_flag_dev};
+    CU_TRY(cudaFuncSetAttribute(k_product<BM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(prod_smem<BM>(2))));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((p.n + TILE_N - 1) / TILE_N * split), static_cast<unsigned>((p.m + BM - 1) / BM));
+    cfg.blockDim = dim3(PROD_THREADS);
+    cfg.dynamicSmemBytes = prod_smem<BM>(split);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned>(split), 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CU_TRY(cudaLaunchKernelEx(&cfg, k_product<BM, T>, map_w, map_a, g));
+    return THRML_OK;
+}
+
+template <class T>
+int32_t product(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
+    const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+    const int64_t tiles = (p.n + TILE_N - 1) / TILE_N * ((p.m + bm - 1) / bm), k_steps = (p.k + KB - 1) / KB;
+    int split = 1;
+    while (split < 8 && tiles * split < 2 * ctx->sm_count && 2 * split <= k_steps) split *= 2;
+    if (bm == 16) return launch_product<16, T>(ctx, stream, p, split);
+    if (bm == 32) return launch_product<32, T>(ctx, stream, p, split);
+    if (bm == 64) return launch_product<64, T>(ctx, stream, p, split);
+    return launch_product<128, T>(ctx, stream, p, split);
+}
+
+int32_t run_product(thrml_ctx* ctx, void* stream, const Product& p) {
+    if (p.m == 0 || p.n == 0) return THRML_OK;
+    return for_type(p.out_type, [&](auto e) { return product<decltype(e)>(ctx, static_cast<cudaStream_t>(stream), p); });
+}
+
+struct Quant {
+    int64_t rows, cols;
+    const void* x;
+    int32_t x_type;
+    int64_t x_pitch;
+    int8_t* q;
+    int64_t q_pitch;
+    float* scale;
+};
+
+int32_t check_quant(const Quant& z) {
+    if (z.rows < 0 || z.rows > INT32_MAX || z.cols < 1 || z.cols > (1 << 30)) return fail(THRML_ERR_INVALID_ARG, "x: the number of rows or columns is out of range");
+    if (!is_float_type(z.x_type)) return fail(THRML_ERR_INVALID_ARG, "x: the element type is not a float type");
+    if (z.x_pitch < z.cols || z.q_pitch < z.cols) return fail(THRML_ERR_INVALID_ARG, "x, q: the pitch is smaller than a row");
+    if (z.rows && (!z.x || !z.q || !z.scale)) return fail(THRML_ERR_INVALID_ARG, "x, q, scale: null pointer");
+    if (!aligned_to(z.x, type_size(z.x_type))) return fail(THRML_ERR_INVALID_ARG, "x: the pointer is not aligned to the element");
+    return THRML_OK;
+}
+
+int32_t run_quant(void* stream, const Quant& z) {
+    if (z.rows == 0) return THRML_OK;
+    const QuantArgs g{z.x, z.x_pitch, z.q, z.q_pitch, z.scale, static_cast<int32_t>(z.cols)};
+    return for_type(z.x_type, [&](auto e) {
+        k_quantize<decltype(e)><<<static_cast<unsigned>(z.rows), QUANT_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(g);
+        CU_TRY(cudaGetLastError());
+        return THRML_OK;
+    });
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t thrml_quantize_rows_i8(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
+                               float* scale) {
+    return guarded(ctx, [&]() -> int32_t {
+        const Quant z{rows, cols, x, x_type, x_pitch, q, q_pitch, scale};
+        if (int32_t rc = check_quant(z)) return rc;
+        return run_quant(stream, z);
+    });
+}
+
+int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* w,
+                        int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch) {
+    return guarded(ctx, [&]() -> int32_t {
+        const Product p{m, n, k, a, a_pitch, a_scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch};
+        if (int32_t rc = check_product(p)) return rc;
+        return run_product(ctx, stream, p);
+    });
+}
+
+int32_t thrml_linear_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
+                        float* scale, const int8_t* w, int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch) {
+    return guarded(ctx, [&]() -> int32_t {
+        const Product p{m, n, k, q, q_pitch, scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch};
+        if (int32_t rc = check_product(p)) return rc;
+        const Quant z{m, k, x, x_type, x_pitch, q, q_pitch, scale};
+        if (int32_t rc = check_quant(z)) return rc;
+        if (m == 0 || n == 0) return THRML_OK;
+        if (int32_t rc = run_quant(stream, z)) return rc;
+        return run_product(ctx, stream, p);
+    });
+}
+
+}  // extern "C"
