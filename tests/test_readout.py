@@ -82,7 +82,7 @@ def rules(T, **kw):
     (dict(logits=None), {}, "null"), (dict(logits=65), {}, "aligned"), (dict(out=None), {}, "null"), (dict(out_pitch=48), {}, "pitch"),
     ({}, dict(history=HERE, history_type=F32, history_ptr=HERE), "index type"), ({}, dict(history=HERE, history_type=I32), "history_ptr"),
     ({}, dict(bias_ids=HERE, bias_values=HERE), "bias_ptr"), ({}, dict(mask=HERE, n_masks=0, mask_pitch=2), "mask"), ({}, dict(mask=HERE, n_masks=1, mask_pitch=1), "mask"),
-    (dict(rows=(1 << 31) - 1, cols=1 << 20, pitch=1 << 20, out_pitch=1 << 20), {}, "too many rows"),
+    (dict(rows=(1 << 31) - 1, cols=1 << 20, pitch=1 << 20, out=4096, out_pitch=1 << 20), {}, "too many rows"),
 ])
 def test_adjust_refuses(T, call, bad, rule, why):
     refused(call("thrml_adjust_logits", *{**GOOD_ADJUST, **bad}.values(), rules(T, **rule)), why)
@@ -106,7 +106,7 @@ def test_draw_refuses(call, bad, why):
 
 GOOD_DISTILL = dict(rows=2, cols=40, logits=HERE, type=F32, pitch=40, top=3, ids=HERE, ids_type=I64, ids_pitch=3, teacher=HERE, teacher_type=BF16, teacher_pitch=3, beta=1.0,
                     weight=None)
-TAILS = {"thrml_distill_loss": dict(loss=HERE, lse=HERE), "thrml_distill_grad": dict(lse=HERE, grad=4096, grad_pitch=40), "thrml_distill_step": dict(loss=HERE, grad=4096, grad_pitch=40)}
+TAILS = {"thrml_distill_loss": dict(loss=HERE, lse=HERE), "thrml_distill_grad": dict(lse=HERE, grad=4096, grad_pitch=40), "thrml_distill_step": dict(loss=HERE, lse=HERE, grad=4096, grad_pitch=40)}
 
 
 @pytest.mark.parametrize("name", TAILS)
@@ -121,8 +121,8 @@ def test_distill_refuses(call, name, bad, why):
 
 @pytest.mark.parametrize("name, bad, why", [
     ("thrml_distill_loss", dict(loss=None), "null"), ("thrml_distill_loss", dict(lse=None), "null"), ("thrml_distill_grad", dict(lse=None), "null"),
-    ("thrml_distill_grad", dict(grad=None), "null"), ("thrml_distill_step", dict(loss=None), "null"), ("thrml_distill_step", dict(grad_pitch=39), "pitch"),
-    ("thrml_distill_step", dict(grad=HERE, grad_pitch=41), "pitch"),
+    ("thrml_distill_grad", dict(grad=None), "null"), ("thrml_distill_step", dict(loss=None), "null"), ("thrml_distill_step", dict(lse=None), "null"), ("thrml_distill_step", dict(grad_pitch=39), "pitch"),
+    ("thrml_distill_step", dict(grad=HERE), "themselves"), ("thrml_distill_grad", dict(grad=HERE), "themselves"),
 ])
 def test_distill_outputs_refused(call, name, bad, why):
     refused(call(name, *GOOD_DISTILL.values(), *{**TAILS[name], **bad}.values()), why)

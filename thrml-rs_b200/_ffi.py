@@ -134,7 +134,7 @@ _SIGNATURES = {
     "thrml_draw_categories": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_uint64, C.c_int64, _P, C.c_int64, _P]),
     "thrml_distill_loss": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P]),
     "thrml_distill_grad": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P, C.c_int64]),
-    "thrml_distill_step": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P, C.c_int64]),
+    "thrml_distill_step": (C.c_int32, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int64, _P, C.c_int32, C.c_int64, C.c_float, _P, _P, _P, _P, C.c_int64]),
 }
 
 

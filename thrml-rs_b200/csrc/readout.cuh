@@ -1,4 +1,4 @@
-// What the readout's translation units share: element types, rows read in 16-byte pieces, block reductions, and the host
+// What the readout's translation units share: element types, rows read in 16-byte pieces, and the host
 // side's call frame (device guard, no exception past the C boundary).
 #pragma once
 #include <cuda_bf16.h>
@@ -47,17 +47,35 @@ __device__ __forceinline__ bool on_16(const void* p) { return (reinterpret_cast<
 
 template <class T>
 __device__ __forceinline__ void unpack_16(const uint4& raw, float (&v)[VEC<T>]) {
-    const T* e = reinterpret_cast<const T*>(&raw);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < VEC<T>; ++i) v[i] = to_float(e[i]);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) v[i] = __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        } else {
+            // a bf16 is the upper half of its f32: shift and mask, where the conversion instruction would run on the pipe that
+            // the exponentials need (a 256 x 131072 draw took 65 us with it)
+            v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
 }
 template <class T>
 __device__ __forceinline__ uint4 pack_16(const float* v) {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < VEC<T>; ++i) e[i] = from_float<T>(v[i]);
-    return raw;
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) w[i] = __float_as_uint(v[i]);
+        else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);  // two conversions in one instruction
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // n values of a row to dst (16 bytes at once where dst allows it).
 template <class T, int N>
@@ -90,28 +108,73 @@ __device__ __forceinline__ void for_row(const T* row, int32_t n, int tid, int th
     }
 }
 
-struct MaxOp {
-    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
-    static constexpr float none = -INFINITY;
-};
-struct SumOp {
-    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
-    static constexpr float none = 0.0f;
-};
-// All threads of the block get the result; `scratch` holds 32 floats.  The order of the additions is fixed.
-template <class Op>
-__device__ __forceinline__ float block_reduce(float x, float* scratch) {
-    const Op op;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, d));
-    __syncthreads();  // the scratch may still be read from an earlier reduction
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : Op::none;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, d));
-    return x;
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
 }
+__device__ __forceinline__ float2 add_2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul_2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 16 bytes to shared memory without passing through registers; the thread that asked for them may read them after its own
+// wait_copies<N>(), which leaves its last N groups in flight.
+__device__ __forceinline__ void copy_16_async(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A row by positions, counted from the last 16-byte boundary at or before its first element: position = element + ahead.  A
+// piece is 16 bytes at a multiple of VEC positions; the row's first and last may hold fewer elements of it.
+template <class T>
+struct Pieces {
+    const T* row;
+    int32_t ahead, end;  // first and last + 1 of the row's positions
+    __device__ __forceinline__ Pieces(const T* r, int32_t cols) : row(r) {
+        ahead = static_cast<int32_t>((reinterpret_cast<uintptr_t>(r) & 15u) / sizeof(T));
+        end = cols + ahead;
+    }
+    __device__ __forceinline__ bool whole(int32_t at) const { return at >= ahead && at + VEC<T> <= end; }
+    // The piece at `at` into `slot`, zeros for what lies outside the row; a whole one is on its way until wait_copies.
+    __device__ __forceinline__ void fetch(uint4* slot, int32_t at) const {
+        if (whole(at)) {
+            copy_16_async(slot, row + (at - ahead));
+        } else {
+            *slot = make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < VEC<T>; ++j)
+                if (at + j >= ahead && at + j < end) reinterpret_cast<T*>(slot)[j] = row[at + j - ahead];
+        }
+    }
+    // The piece to the same place of another row (16 bytes at once where `wide`), except the elements marked in `skip`.
+    __device__ __forceinline__ void store(T* to, int32_t at, const uint4& raw, bool wide, uint32_t skip) const {
+        if (wide && whole(at) && !skip) {
+            *reinterpret_cast<uint4*>(to + (at - ahead)) = raw;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC<T>; ++j)
+                if (at + j >= ahead && at + j < end && !((skip >> j) & 1u)) to[at + j - ahead] = reinterpret_cast<const T*>(&raw)[j];
+        }
+    }
+    // Whether pieces of `to` lie on 16-byte boundaries as the row's do.
+    __device__ __forceinline__ bool same_phase(const T* to) const { return ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(row)) & 15u) == 0; }
+};
 
 // ---- host side
 inline bool is_float_type(int32_t t) { return t == THRML_F32 || t == THRML_BF16 || t == THRML_F16; }

@@ -1,8 +1,12 @@
 // The readout's operators on logits: the rules of a generation step, the draw of a category, and the distillation loss with
 // its gradient.  One row = one sequence (or chain) of up to 2^30 categories; sums, softmax statistics and scores are held in
 // f32 or f64, and each output is rounded once to its own type.
+#include <algorithm>
+#include <cstddef>
+
 #include "device_math.cuh"
 #include "readout.cuh"
+#include "tensor_core.cuh"
 
 using namespace thrml;
 using namespace thrml::readout;
@@ -12,93 +16,255 @@ namespace {
 constexpr int64_t MAX_COLS = 1 << 30;  // indices inside a row stay in 32 bits
 constexpr int TOP_MAX = 1024;          // listed teacher entries held in shared memory
 constexpr uint32_t TAG_DRAW = 0x44524157u;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Floats as integers in the same order, for integer maxima.
+__device__ __forceinline__ int32_t ordered(float x) {
+    const int32_t b = __float_as_int(x);
+    return b < 0 ? b ^ 0x7fffffff : b;
+}
+__device__ __forceinline__ float from_ordered(int32_t b) { return __int_as_float(b < 0 ? b ^ 0x7fffffff : b); }
+
+// 16 bytes of -infinity.
+template <class T>
+__device__ __forceinline__ uint4 nothing_16() {
+    constexpr uint32_t w = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+}
 
 // ---------------------------------------------------------------------------------------------------------
 // Rules on logits.
+//
+// Bound by memory: every logit is read and written once.  A CTA copies a share of a row into shared memory, ADJUST_PIECES 16-byte
+// pieces a thread, in flight together; meanwhile it counts there those of the row's tokens that fall into the share (integer atomics, so the counts do not depend on their order).  A count has 16 bits, and 32 in rows of 2^15 tokens
+// or more, which are done half a share at a time.  Every CTA of a row reads the whole history, from L2 after the first.
+// Categories with a bias are finished by a thread of their own, before the pass over the share, which leaves out what a bitmap
+// marks.  Measured and dropped for 256 rows of 131072 bf16 with 3000 tokens each: the few named categories in a kernel of
+// their own behind a plain copy, 77 us (their scattered 2-byte writes cost more than they are); for 16 rows with 60000
+// tokens, the history read once per row with atomics into the shared memory of the CTA that holds the category, 137 us, since
+// few categories take most of the tokens.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int ADJUST_THREADS = 256, ADJUST_SLICE = 8192;
-constexpr uint32_t IN_PROMPT = 0x80000000u;
+constexpr int ADJUST_THREADS = 512, ADJUST_PIECES = 4;
+template <class T>
+constexpr int ADJUST_SHARE = ADJUST_THREADS * ADJUST_PIECES * VEC<T>;  // most positions of a CTA
 
 struct AdjustArgs {
     const void* logits;
     void* out;
     int64_t pitch, out_pitch;
-    int32_t cols, slices;
+    int32_t cols, share, per_row, count_words;  // positions of a row per CTA, CTAs per row, words of counts
     thrml_logit_rules rules;
 };
 
-// A CTA takes one slice of one row.  The history's tokens that fall into the slice are counted in shared memory (integer
-// atomics: the counts do not depend on their order), the biases are summed there, and one pass over the slice reads, adjusts
-// and writes the logits.
+// -infinity where the bit is 0.
 template <class T>
-__global__ void __launch_bounds__(ADJUST_THREADS) k_adjust(const AdjustArgs g) {
-    extern __shared__ uint32_t adjust_smem[];
+__device__ __forceinline__ uint4 close_16(const uint4& raw, uint32_t open) {
+    const uint4 none = nothing_16<T>();
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4) x[i] = (open >> i) & 1u ? w[i] : none.x;
+        else {
+            const uint32_t keep = (((open >> (2 * i)) & 1u) | ((open >> (2 * i) & 2u) << 15)) * 0xffffu;  // bits 0 and 16 to all of their halves
+            x[i] = (w[i] & keep) | (none.x & ~keep);
+        }
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
+// What the penalties make of a logit that was seen, `told` times behind the prompt.
+struct Penalties {
+    float repetition, per_repetition, frequency, presence;
+    __device__ __forceinline__ float operator()(float x, uint32_t told) const {
+        x *= x > 0.0f ? per_repetition : repetition;
+        return told ? x - fmaf(frequency, static_cast<float>(told), presence) : x;
+    }
+};
+
+// Counts of BITS bits, packed in words, the highest for "in the prompt".
+template <int BITS>
+struct Counts {
+    static constexpr int PER_WORD = 32 / BITS;
+    static constexpr uint32_t IN_PROMPT = 1u << (BITS - 1), ALL = BITS == 32 ? 0xffffffffu : (1u << BITS) - 1u;
+    uint32_t* words;
+    __device__ __forceinline__ static int shift(uint32_t i) { return BITS * (i % PER_WORD); }
+    __device__ __forceinline__ void prompt(uint32_t i) const { atomicOr(words + i / PER_WORD, IN_PROMPT << shift(i)); }
+    __device__ __forceinline__ void told(uint32_t i) const { atomicAdd(words + i / PER_WORD, 1u << shift(i)); }
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return (words[i / PER_WORD] >> shift(i)) & ALL; }
+};
+
+// f(place) for each token that lies in [low, low + n).
+template <class I, class F>
+__device__ __forceinline__ void each_token(const I* history, int64_t h0, int64_t h1, int32_t low, uint32_t n, F f) {
+    using U = typename std::make_unsigned<I>::type;
+    constexpr int AT_ONCE = 4;
+    while (h0 < h1) {
+        const int32_t len = static_cast<int32_t>(min(h1 - h0, int64_t{1} << 30));
+        const I* h = history + h0;
+#pragma unroll 1
+        for (int32_t i = threadIdx.x; i < len; i += AT_ONCE * ADJUST_THREADS) {
+            U at[AT_ONCE];
+#pragma unroll
+            for (int t = 0; t < AT_ONCE; ++t) at[t] = i + t * ADJUST_THREADS < len ? static_cast<U>(h[i + t * ADJUST_THREADS]) - static_cast<U>(I{low}) : n;
+#pragma unroll
+            for (int t = 0; t < AT_ONCE; ++t)
+                if (at[t] < n) f(static_cast<uint32_t>(at[t]));  // a token below low has wrapped to beyond n
+        }
+        h0 += len;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_constant__ AdjustArgs g) {
+    constexpr int V = VEC<T>;
+    extern __shared__ uint4 adjust_smem[];
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x / g.slices;
-    const int32_t k0 = static_cast<int32_t>(blockIdx.x % g.slices) * ADJUST_SLICE, n = min(ADJUST_SLICE, g.cols - k0);
     const thrml_logit_rules& ru = g.rules;
-    uint32_t* count = adjust_smem;
-    float* bias = reinterpret_cast<float*>(adjust_smem + (ru.history ? ADJUST_SLICE : 0));
+    const int64_t row = g.per_row == 1 ? blockIdx.x : blockIdx.x / g.per_row;
+    const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
+    T* out = static_cast<T*>(g.out) + row * g.out_pitch;
+    const Pieces<T> pieces(logits, g.cols);
+    const int32_t ahead = pieces.ahead;
+    const int32_t from = static_cast<int32_t>(blockIdx.x - row * g.per_row) * g.share, to = min(pieces.end, from + g.share);
+    if (from >= to) return;
+    uint4* tile = adjust_smem;  // a thread's piece s at s * ADJUST_THREADS + tid
+    uint4* counts = tile + ADJUST_PIECES * ADJUST_THREADS;                                                                       // [share] of 16 bits, when there are histories
+    uint32_t* biased = reinterpret_cast<uint32_t*>(counts) + (ru.history ? g.count_words : 0);  // [share] bits, when there are biases
 
     const int64_t h0 = ru.history ? ru.history_ptr[row] : 0, h1 = ru.history ? ru.history_ptr[row + 1] : 0;
     const int64_t b0 = ru.bias_ids ? ru.bias_ptr[row] : 0, b1 = ru.bias_ids ? ru.bias_ptr[row + 1] : 0;
-    const bool has_history = h1 > h0, has_bias = b1 > b0;
-    if (has_history)
-        for (int i = tid; i < n; i += ADJUST_THREADS) count[i] = 0;
-    if (has_bias)
-        for (int i = tid; i < n; i += ADJUST_THREADS) bias[i] = 0.0f;
-    __syncthreads();
-    if (has_history) {
-        const int64_t prompt_end = h0 + (ru.n_prompt ? max(ru.n_prompt[row], 0) : 0);
-        for (int64_t i = h0 + tid; i < h1; i += ADJUST_THREADS) {
-            const int64_t at = load_as_int(ru.history, ru.history_type, i) - k0;
-            if (at >= 0 && at < n) {
-                if (i < prompt_end) atomicOr(count + at, IN_PROMPT);
-                else atomicAdd(count + at, 1u);
-            }
-        }
-    }
-    if (has_bias) {
-        // the first entry of a run of equal ids adds the run up in its order
-        for (int64_t i = b0 + tid; i < b1; i += ADJUST_THREADS) {
-            const int32_t id = ru.bias_ids[i], at = id - k0;
-            if (id < 0 || at < 0 || at >= n || (i > b0 && ru.bias_ids[i - 1] == id)) continue;
-            float sum = ru.bias_values[i];
-            for (int64_t j = i + 1; j < b1 && ru.bias_ids[j] == id; ++j) sum += ru.bias_values[j];
-            atomicAdd(bias + at, sum);  // one addend unless the ids are not in order
-        }
-    }
-    __syncthreads();
-
-    const float repetition = ru.repetition ? ru.repetition[row] : 1.0f, frequency = ru.frequency ? ru.frequency[row] : 0.0f,
-                presence = ru.presence ? ru.presence[row] : 0.0f;
+    auto place = [&](int s) { return from + (s * ADJUST_THREADS + tid) * V; };
+    for (int s = 0; s < ADJUST_PIECES; ++s)
+        if (place(s) < to) pieces.fetch(tile + s * ADJUST_THREADS + tid, place(s));
+    commit_copies();
+    const int32_t n_bias = static_cast<int32_t>(b1 - b0);
+    const bool has_history = h1 > h0, has_bias = n_bias > 0;
+    const int32_t* ids = ru.bias_ids + b0;
+    const int64_t split = has_history && ru.n_prompt ? min(h1, h0 + max(ru.n_prompt[row], 0)) : h0;
+    const float repetition = ru.repetition ? ru.repetition[row] : 1.0f;
+    const Penalties penalise{repetition, __fdiv_rn(1.0f, repetition),  // one division a row instead of one a category: 1.5 steps of f32 at most
+                             ru.frequency ? ru.frequency[row] : 0.0f, ru.presence ? ru.presence[row] : 0.0f};
     const int64_t m = !ru.mask ? -1 : ru.mask_rows ? ru.mask_rows[row] : row;
     const uint32_t* mask = ru.mask && m >= 0 && m < ru.n_masks ? ru.mask + m * ru.mask_pitch : nullptr;
-    const T* in = static_cast<const T*>(g.logits) + row * g.pitch + k0;
-    T* out = static_cast<T*>(g.out) + row * g.out_pitch + k0;
-    for_row<T>(in, n, tid, ADJUST_THREADS, [&](int32_t i, const float* v, auto cnt) {
-        constexpr int N = decltype(cnt)::value;
-        float x[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            x[j] = v[j];
-            const uint32_t c = has_history ? count[i + j] : 0u;
-            if (c) {
-                x[j] = x[j] > 0.0f ? __fdiv_rn(x[j], repetition) : x[j] * repetition;
-                const uint32_t told = c & ~IN_PROMPT;
-                if (told) x[j] = x[j] - frequency * static_cast<float>(told) - presence;
-            }
-            if (has_bias) x[j] += bias[i + j];
-            if (mask && !((mask[(k0 + i + j) >> 5] >> ((k0 + i + j) & 31)) & 1u)) x[j] = -INFINITY;
+    const bool wide = pieces.same_phase(out);
+    float logit = 0.0f;  // of the first bias entry that this thread finishes, read early
+    if (has_bias) {
+        for (int i = tid; i < g.share / 32; i += ADJUST_THREADS) biased[i] = 0u;
+        __syncthreads();
+        for (int32_t e = tid; e < n_bias; e += ADJUST_THREADS) {
+            const uint32_t at = ids[e] - (from - ahead);
+            if (ids[e] < 0 || at >= static_cast<uint32_t>(to - from)) continue;
+            atomicOr(biased + (at >> 5), 1u << (at & 31));
+            if (e == tid) logit = to_float(logits[ids[e]]);
         }
-        store_n<T>(out + i, x, cnt);
-    });
+    }
+
+    // Pieces s0 .. s1 of each thread, the positions [begin, stop), with counts of BITS bits.
+    auto pass = [&](auto bits, int s0, int s1, int32_t begin, int32_t stop) {
+        constexpr int BITS = decltype(bits)::value;
+        const Counts<BITS> count{reinterpret_cast<uint32_t*>(counts)};
+        if (has_history) {
+            for (int i = tid; i < (stop - begin + 128 / BITS - 1) / (128 / BITS); i += ADJUST_THREADS) counts[i] = make_uint4(0u, 0u, 0u, 0u);
+            __syncthreads();
+            // `low` is the category at `begin`; below 0 (the first CTA's, when ahead > 0) lie no categories
+            const int32_t low = max(begin - ahead, 0);
+            const uint32_t first = low + ahead - begin, n = static_cast<uint32_t>(stop - ahead - low);
+            auto each = [&](auto* history) {
+                each_token(history, h0, split, low, n, [&](uint32_t i) { count.prompt(first + i); });
+                each_token(history, split, h1, low, n, [&](uint32_t i) { count.told(first + i); });
+            };
+            if (ru.history_type == THRML_I64) each(static_cast<const int64_t*>(ru.history));
+            else each(static_cast<const int32_t*>(ru.history));
+        }
+        wait_copies<0>();  // before any write, which may be in place
+        __syncthreads();
+        if (has_bias) {
+            // the first of a category's entries finishes it for all of them
+            for (int32_t e = tid; e < n_bias; e += ADJUST_THREADS) {
+                const int32_t id = ids[e];
+                const uint32_t at = id - (begin - ahead);
+                if (id < 0 || at >= static_cast<uint32_t>(stop - begin) || (e > 0 && ids[e - 1] == id)) continue;
+                float sum = ru.bias_values[b0 + e];
+                for (int32_t i = e + 1; i < n_bias && ids[i] == id; ++i) sum += ru.bias_values[b0 + i];
+                float x = e == tid ? logit : to_float(logits[id]);
+                if (has_history) {
+                    const uint32_t c = count.at(at);
+                    if (c) x = penalise(x, c & ~Counts<BITS>::IN_PROMPT);
+                }
+                x += sum;
+                if (mask && !((mask[id >> 5] >> (id & 31)) & 1u)) x = -INFINITY;
+                out[id] = from_float<T>(x);
+            }
+        }
+#pragma unroll 1
+        for (int s = s0; s < s1; ++s) {
+            const int32_t at = place(s), k = at - ahead;
+            if (at >= stop) break;
+            uint4& raw = tile[s * ADJUST_THREADS + tid];
+            if (has_history) {
+                constexpr int WORDS = V * BITS / 32;  // of a piece's counts: 2, 4 or 8
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(counts) + (at - begin) / Counts<BITS>::PER_WORD;
+                uint32_t some = 0u;  // a bit per word
+#pragma unroll
+                for (int j = 0; j < WORDS; j += 2) {
+                    const uint2 q = *reinterpret_cast<const uint2*>(w + j);
+                    some |= (q.x ? 1u << j : 0u) | (q.y ? 2u << j : 0u);
+                }
+                // A logit is rounded to its type once: what is penalised and not biased is final; what is biased is not written below.
+                while (some) {
+                    const int word = __ffs(some) - 1;
+                    some &= some - 1u;
+#pragma unroll
+                    for (int h = 0; h < Counts<BITS>::PER_WORD; ++h) {
+                        const int j = word * Counts<BITS>::PER_WORD + h;
+                        const uint32_t c = (w[word] >> Counts<BITS>::shift(h)) & Counts<BITS>::ALL;
+                        T& x = reinterpret_cast<T*>(&raw)[j];
+                        if (c) x = from_float<T>(penalise(to_float(x), c & ~Counts<BITS>::IN_PROMPT));
+                    }
+                }
+            }
+            uint4 bits = raw;
+            if (mask) {
+                const int32_t k0 = max(k, 0);  // the first piece of a row may begin before it
+                uint32_t open = mask[k0 >> 5] >> (k0 & 31);
+                if ((k0 & 31) + V > 32 && ((k0 >> 5) + 1) * 32 < g.cols) open |= mask[(k0 >> 5) + 1] << (32 - (k0 & 31));
+                bits = close_16<T>(bits, open << (k0 - k));
+            }
+            const uint32_t done = has_bias ? biased[(at - from) >> 5] >> ((at - from) & 31) & ((1u << V) - 1u) : 0u;  // V positions lie in one word
+            pieces.store(out, at, bits, wide, done);
+        }
+    };
+    if (h1 - h0 < 1 << 15) {
+        pass(Count<16>{}, 0, ADJUST_PIECES, from, to);
+    } else {
+        const int32_t half = from + ADJUST_PIECES / 2 * ADJUST_THREADS * V;
+        pass(Count<32>{}, 0, ADJUST_PIECES / 2, from, min(to, half));
+        if (half < to) {
+            __syncthreads();  // the counts are read
+            pass(Count<32>{}, ADJUST_PIECES / 2, ADJUST_PIECES, half, to);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // The draw of a category.
+//
+// score = beta l - log(-log u) exceeds a bound B exactly when -ln u < exp(beta l - B), and -ln u >= 1 - u: so a category whose
+// 1 - u lies above exp(beta l - B) cannot be the largest once B is a score that some category reaches.  That test costs one
+// hardware exponential and no logarithm, and nearly every category fails it.  The ones that pass get their score in f64
+// (where two scores that f32 cannot tell apart have an order), which decides.  B starts from approximate scores of each
+// thread's first categories, lowered by more than their error, and rises with the scores found, shared in the CTA.
+// Bound by instruction issue: ten rounds of the generator serve four categories.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int DRAW_THREADS = 512;
+constexpr int DRAW_THREADS = 256, DRAW_GROUP = 8;  // categories of a thread's turn: two generator calls
+constexpr int DRAW_AHEAD = 4;                      // turns whose logits are on their way
 
 struct DrawArgs {
     const void* logits;
@@ -106,7 +272,7 @@ struct DrawArgs {
     const float* noise;
     int64_t* out;
     int64_t pitch, noise_pitch;
-    int32_t cols;
+    int32_t cols, share, per_row;  // categories per CTA, CTAs (= a cluster) per row
     uint32_t row_offset;
     PhiloxRoundKeys rk;
 };
@@ -123,32 +289,144 @@ struct Best {
     }
 };
 
-// One CTA per row; every score in f64.
+// The scores in f64 of those of DRAW_GROUP categories that reach the bound, out of line: few turns have any.
 template <class T>
-__global__ void __launch_bounds__(DRAW_THREADS) k_draw(const DrawArgs g) {
-    __shared__ double sh_score[DRAW_THREADS / 32];
-    __shared__ int32_t sh_k[DRAW_THREADS / 32];
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
+__device__ __noinline__ void weigh(Best& best, int32_t* bound, const DrawArgs& g, const T* logits, const float* noise, float beta, int64_t row, int32_t k, int32_t to) {
+    for (int h = 0; h < DRAW_GROUP && k + h < to; h += 4) {
+        U4 w{};
+        if (!noise && beta != INFINITY) w = philox4x32_10_rk(g.row_offset + static_cast<uint32_t>(row), 0u, static_cast<uint32_t>(k + h) >> 2, TAG_DRAW, g.rk);
+        for (int j = h; j < h + 4 && k + j < to; ++j) {
+            const float l = to_float(logits[k + j]);
+            if (!(l > -INFINITY)) continue;  // masked, or not a number
+            double score = l;
+            if (beta != INFINITY) {
+                const float u = noise ? noise[k + j] : u23_open(pick(w, j - h));
+                const float b = from_ordered(*static_cast<volatile int32_t*>(bound));
+                if (fmaf(beta, l, -__logf(1.0f - u)) + 1e-2f + 1e-5f * (fabsf(beta * l) + fabsf(b)) < b) continue;  // -ln u >= 1 - u, once more for each
+                score = __dsub_rn(__dmul_rn(beta, l), log(-log(static_cast<double>(u))));
+            }
+            best.take(score, k + j);
+            if (score > -INFINITY) atomicMax(bound, ordered(__double2float_rd(score)));
+        }
+    }
+}
+
+template <class T, bool GIVEN>
+__global__ void __launch_bounds__(DRAW_THREADS, 5) k_draw(const __grid_constant__ DrawArgs g) {
+    __shared__ Best warps[DRAW_THREADS / 32], ctas[8];
+    __shared__ int32_t bound;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int64_t row = blockIdx.x / g.per_row;
+    const int32_t part = static_cast<int32_t>(blockIdx.x % g.per_row), from = part * g.share, to = min(g.cols, from + g.share);
+    if (g.per_row > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const float beta = g.beta ? g.beta[row] : 1.0f;
     const bool greedy = beta == INFINITY;
     const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
-    const float* noise = g.noise ? g.noise + row * g.noise_pitch : nullptr;
+    const float* noise = GIVEN ? g.noise + row * g.noise_pitch : nullptr;
+    const bool wide = on_16(logits + from);  // shares are multiples of DRAW_GROUP
+    const float b2 = beta * LOG2E;
+
+    // The logits of a turn, through shared memory, DRAW_AHEAD turns ahead; a thread reads what it asked for.  What lies behind the
+    // share is masked.
+    constexpr int PIECES = DRAW_GROUP / VEC<T>;
+    __shared__ uint4 ring[DRAW_AHEAD][PIECES][DRAW_THREADS];
+    auto fetch = [&](int32_t k, int turn) {
+        uint4(*slot)[DRAW_THREADS] = ring[turn % DRAW_AHEAD];
+        if (k < to) {
+            if (wide && k + DRAW_GROUP <= to) {
+#pragma unroll
+                for (int h = 0; h < PIECES; ++h) copy_16_async(&slot[h][tid], logits + k + h * VEC<T>);
+            } else {
+                for (int h = 0; h < PIECES; ++h) {
+                    slot[h][tid] = nothing_16<T>();
+                    for (int j = 0; j < VEC<T>; ++j)
+                        if (k + h * VEC<T> + j < to) reinterpret_cast<T*>(&slot[h][tid])[j] = logits[k + h * VEC<T> + j];
+                }
+            }
+        }
+        commit_copies();
+    };
+    auto logits_of = [&](int turn, float (&l)[DRAW_GROUP]) {
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+            float v[VEC<T>];
+            unpack_16<T>(ring[turn % DRAW_AHEAD][h][tid], v);
+#pragma unroll
+            for (int j = 0; j < VEC<T>; ++j) l[h * VEC<T> + j] = v[j];
+        }
+    };
+    // Their uniforms.  From the key: 1 + n 2^-23, where u = (n + 1/2) 2^-23; given: u.
+    auto draw = [&](int32_t k, float (&f)[DRAW_GROUP]) {
+        if (greedy) return;
+        if (GIVEN) {
+#pragma unroll
+            for (int j = 0; j < DRAW_GROUP; ++j) f[j] = k + j < to ? noise[k + j] : 0.0f;
+        } else {
+#pragma unroll
+            for (int h = 0; h < DRAW_GROUP; h += 4) {
+                const U4 w = philox4x32_10_rk(g.row_offset + static_cast<uint32_t>(row), 0u, static_cast<uint32_t>(k + h) >> 2, TAG_DRAW, g.rk);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[h + j] = __uint_as_float(__funnelshift_r(pick(w, j), 0x7fu, 9));  // the exponent of 1, then n
+            }
+        }
+    };
+
     Best best{0.0, -1};
     if (beta >= 0.0f) {
-        for (int32_t k = 4 * tid; k < g.cols; k += 4 * DRAW_THREADS) {
-            U4 words{};
-            if (!noise && !greedy) words = philox4x32_10_rk(g.row_offset + static_cast<uint32_t>(row), 0u, static_cast<uint32_t>(k) >> 2, TAG_DRAW, g.rk);
-            for (int j = 0; j < 4 && k + j < g.cols; ++j) {
-                const float l = to_float(logits[k + j]);
-                if (!(l > -INFINITY)) continue;  // masked, or not a number
-                double score = l;
+        // A first bound, from each thread's first categories.
+        float first = -INFINITY;
+        const int32_t k0 = from + tid * DRAW_GROUP, step = DRAW_THREADS * DRAW_GROUP;
+        for (int t = 0; t < DRAW_AHEAD; ++t) fetch(k0 + t * step, t);
+        wait_copies<DRAW_AHEAD - 1>();
+        if (k0 < to) {
+            float l[DRAW_GROUP], f[DRAW_GROUP];
+            draw(k0, f);
+            logits_of(0, l);
+#pragma unroll
+            for (int j = 0; j < (GIVEN ? DRAW_GROUP : 4); ++j) {
+                float s = l[j];
                 if (!greedy) {
-                    const double u = noise ? noise[k + j] : u23_open(pick(words, j));
-                    score = __dsub_rn(__dmul_rn(beta, l), log(-log(u)));
+                    const float u = GIVEN ? f[j] : (f[j] - 1.0f) + 0x1p-24f;
+                    s = fmaf(beta, l[j], -__logf(-__logf(u)));
+                    s -= 1e-2f + 1e-5f * fabsf(s);
+                    if (!(u < 0.9f)) s = -INFINITY;  // up to there the two logarithms are good to 1e-2 by far
                 }
-                best.take(score, k + j);
+                if (l[j] > -INFINITY && s < INFINITY) first = fmaxf(first, s);
             }
+        }
+        for (int d = 16; d; d >>= 1) first = fmaxf(first, __shfl_xor_sync(0xffffffffu, first, d));
+        if (tid == 0) bound = ordered(-INFINITY);
+        __syncthreads();
+        if (lane == 0) atomicMax(&bound, ordered(first));
+        __syncthreads();
+        for (int32_t k = k0, turn = 0; k < to; k += step, ++turn) {
+            float l[DRAW_GROUP], f[DRAW_GROUP];
+            wait_copies<DRAW_AHEAD - 1>();
+            logits_of(turn, l);
+            fetch(k + DRAW_AHEAD * step, turn);  // into the place just read
+            const float b = from_ordered(*static_cast<volatile int32_t*>(&bound));
+            bool some = false;
+            if (greedy) {
+#pragma unroll
+                for (int j = 0; j < DRAW_GROUP; ++j) some |= l[j] >= b;
+            } else {
+                draw(k, f);
+                // c = the bound in base 2, lowered by the roundings of c and of beta l log2(e), 2^-22 of their sizes (a category 60 or
+                // more below c is out of reach of them), and by the exponential's error
+                const float c = b * LOG2E, low = b == INFINITY ? b : c - (fabsf(c) + 60.0f) * 0x1p-21f - 1e-5f;
+#pragma unroll
+                for (int j = 0; j < DRAW_GROUP; j += 2) {
+                    const float2 a = fma_2(make_float2(l[j], l[j + 1]), both(b2), both(-low)), e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+                    // 1 - u = 2 - f - 2^-24 for the key's; the rounding of 2 - 2^-22 - e is covered.  What is no number passes here.
+                    if (GIVEN) {
+                        some |= !(1.0f - f[j] > e.x) | !(1.0f - f[j + 1] > e.y);
+                    } else {
+                        const float2 least = fma_2(e, both(-1.0f), both(2.0f - 0x1p-22f));
+                        some |= !(f[j] < least.x) | !(f[j + 1] < least.y);
+                    }
+                }
+            }
+            if (some) weigh<T>(best, &bound, g, logits, noise, beta, row, k, to);
         }
     }
     for (int d = 16; d; d >>= 1) {
@@ -156,21 +434,46 @@ __global__ void __launch_bounds__(DRAW_THREADS) k_draw(const DrawArgs g) {
         const int32_t k = __shfl_xor_sync(0xffffffffu, best.k, d);
         best.take(s, k);
     }
-    if ((tid & 31) == 0) {
-        sh_score[tid >> 5] = best.score;
-        sh_k[tid >> 5] = best.k;
-    }
+    if (lane == 0) warps[tid >> 5] = best;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < DRAW_THREADS / 32; ++w) best.take(sh_score[w], sh_k[w]);
-        g.out[row] = best.k;
+    if (tid < 32) {
+        best = warps[tid % (DRAW_THREADS / 32)];
+        for (int d = 16; d; d >>= 1) {
+            const double s = __shfl_xor_sync(0xffffffffu, best.score, d);
+            const int32_t k = __shfl_xor_sync(0xffffffffu, best.k, d);
+            best.take(s, k);
+        }
     }
+    if (g.per_row > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the row's first CTA has started
+        if (tid == 0) {
+            const uint32_t at = dense::peer_addr(dense::smem_u32(&ctas[part]), 0);
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(best.score) : "memory");
+            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at + static_cast<uint32_t>(offsetof(Best, k))), "r"(best.k) : "memory");
+        }
+        dense::cluster_sync_all();
+        for (int c = 1; c < g.per_row; ++c) best.take(ctas[c].score, ctas[c].k);
+    }
+    if (part == 0 && tid == 0) g.out[row] = best.k;
 }
 
 // ---------------------------------------------------------------------------------------------------------
 // Distillation.
+//
+// With z = beta * logits, the row's softmax q = exp(z - lse) and the teacher's p over the listed entries:
+//     loss = sum_j p_j (log p_j - z_id(j) + lse),   d loss / d logits = beta (q - p).
+// Two kernels.  k_softmax streams the rows: lse (loss), weight * beta * q from a given lse (grad), or both (step), where the
+// second pass finds the row in L2 (a CTA, or each of a cluster of up to eight, has 64 KB of it).  k_listed then has one warp, or
+// four, for each row's list: the loss, and the few gradients that p changes.  What was measured and dropped (4096 x 32768 bf16,
+// 64 listed, a step): rows held in registers or in shared memory, once per CTA or in rings of two and three rows, the
+// list inside the same kernel: 125 to 200 us, since the list's chain of small loads, each as slow as a full memory system
+// makes it, held up the rows.
+// Per element one multiply-add and one hardware exponential a pass, in base 2, two elements an instruction where there is
+// one; probabilities below 2^-126 count as 0.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int DISTILL_THREADS = 512;
+constexpr int SOFTMAX_THREADS = 256;
+constexpr int64_t SOFTMAX_BYTES = 64 << 10;  // of a row per CTA
+constexpr int LIST_WARPS = 4;
 enum Distill { LOSS, GRAD, STEP };
 
 struct DistillArgs {
@@ -182,119 +485,378 @@ struct DistillArgs {
     float* loss;
     float* lse_out;
     void* grad;
-    int64_t pitch, ids_pitch, teacher_pitch, grad_pitch;
+    int64_t rows, pitch, ids_pitch, teacher_pitch, grad_pitch;
     int32_t cols, top, ids_type, teacher_type;
     float beta;
+    int32_t share, per_row;  // positions of a row per CTA, CTAs per row
 };
 
-// The teacher's side of one row, in shared memory.
-struct Listed {
-    int32_t id[TOP_MAX];   // -1 = not listed
-    float p[TOP_MAX];      // softmax over the listed entries
-    float z[TOP_MAX];      // beta times the student's logit there
-    float scratch[32];
-    int any;
+// Where beta times the largest logit is FAR or more, neighbouring values of the type lie so far apart that a category either
+// is the largest or has no weight; there (rows whose mask is the type's lowest value and leaves nothing) the scaled logits could
+// overflow, and are not formed.
+constexpr float FAR = 0x1p100f;
+__device__ __forceinline__ bool is_far(float z) { return !(fabsf(z) < FAR); }
+__device__ __forceinline__ float far_weight(float l, float most) { return l != l ? l : l == most ? (most == INFINITY ? NAN : most == -INFINITY ? 0.0f : 1.0f) : 0.0f; }
+
+// A part of a softmax's sum: 2^(b2 l - b2 ref) over its logits l, with b2 ref rounded.  ref is one of the logits or above them,
+// the largest where it is far; -infinity while there is nothing.
+struct Partial {
+    float ref, sum;
+    __device__ __forceinline__ void join(Partial o, float b2) {
+        const float top = fmaxf(ref, o.ref);
+        // a part at -infinity adds nothing; its sum is 0, or NaN when it has met one
+        const float a = ref == top || ref == -INFINITY ? 1.0f : step(ref, top, b2);
+        const float b = o.ref == top || o.ref == -INFINITY ? 1.0f : step(o.ref, top, b2);
+        sum = fmaf(sum, a, o.sum * b);
+        ref = top;
+    }
+    // From one rounded b2 ref to the other; differences first where the products could overflow (the result is 0 there).
+    static __device__ __forceinline__ float step(float from, float to, float b2) {
+        const float a = __fmul_rn(from, b2), b = __fmul_rn(to, b2);
+        return exp2_fast(fabsf(a) < INFINITY && fabsf(b) < INFINITY ? a - b : (from - to) * b2);
+    }
 };
 
-// Fills `L` (all threads of the block).
+// One CTA's share of a row: whole pieces of 16 bytes from `first` on, and up to VEC - 1 elements before and behind them.
 template <class T>
-__device__ __forceinline__ void list_teacher(Listed& L, const DistillArgs& g, int64_t row, const T* logits) {
-    if (threadIdx.x == 0) L.any = 0;
-    float most = -INFINITY;
-    bool some = false;
-    __syncthreads();
-    for (int j = threadIdx.x; j < g.top; j += blockDim.x) {
-        const int64_t id = load_as_int(g.ids, g.ids_type, row * g.ids_pitch + j);
-        const float t = g.beta * load_as_float(g.teacher, g.teacher_type, row * g.teacher_pitch + j);
-        const bool listed = id >= 0 && id < g.cols && !(t == -INFINITY);
-        L.id[j] = listed ? static_cast<int32_t>(id) : -1;
-        L.p[j] = t;
-        L.z[j] = listed ? g.beta * to_float(logits[id]) : 0.0f;
-        if (listed) {
-            most = fmaxf(most, t);
-            some = true;
+struct Share {
+    const T* row;
+    int32_t head, first, pieces, tail, stop;  // elements [head, first), pieces from first, elements [tail, stop)
+    __device__ __forceinline__ Share(const T* r, int32_t cols, int32_t from, int32_t share) : row(r) {
+        const Pieces<T> p(r, cols);
+        const int32_t to = min(p.end, from + share);
+        head = max(from - p.ahead, 0);
+        stop = max(to - p.ahead, head);
+        first = min(from < p.ahead ? from + VEC<T> - p.ahead : head, stop);
+        pieces = (stop - first) / VEC<T>;
+        tail = first + pieces * VEC<T>;
+    }
+    __device__ __forceinline__ uint4 piece(int32_t i) const { return *reinterpret_cast<const uint4*>(row + first + i * VEC<T>); }
+};
+
+// The larger of the even and of the odd elements of 16 bytes.  A bf16 in the upper half of a word is compared with the lower half
+// as further fraction bits, which do not change which is the largest; upper() drops them.  What is no number, or is made one by
+// those bits, gives way (an infinity that is missed so shows in the sum).
+template <class T>
+__device__ __forceinline__ void larger_16(float& a, float& b, const uint4& raw) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            a = fmaxf(a, __uint_as_float(w[i]));
+            b = fmaxf(b, __uint_as_float(w[i] << 16));
+        } else if constexpr (std::is_same<T, float>::value) {
+            if (i & 1) b = fmaxf(b, __uint_as_float(w[i]));
+            else a = fmaxf(a, __uint_as_float(w[i]));
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            a = fmaxf(a, f.x), b = fmaxf(b, f.y);
         }
     }
-    if (some) L.any = 1;
-    most = block_reduce<MaxOp>(most, L.scratch);
-    float total = 0.0f;
-    for (int j = threadIdx.x; j < g.top; j += blockDim.x) {
-        L.p[j] = L.id[j] >= 0 ? expf(L.p[j] - most) : 0.0f;
-        total += L.p[j];
-    }
-    total = block_reduce<SumOp>(total, L.scratch);
-    for (int j = threadIdx.x; j < g.top; j += blockDim.x) L.p[j] = L.p[j] / total;
-    __syncthreads();
+}
+template <class T>
+__device__ __forceinline__ float upper(float a) {
+    return std::is_same<T, __nv_bfloat16>::value ? __uint_as_float(__float_as_uint(a) & 0xffff0000u) : a;
+}
+__device__ __forceinline__ float warp_max(float x) { return from_ordered(__reduce_max_sync(0xffffffffu, ordered(x))); }
+__device__ __forceinline__ float warp_total(float x) {
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
 }
 
-// One CTA per row.  LOSS: maximum and sum of the softmax in one pass, then the loss over the listed entries.  GRAD: one pass
-// that writes weight * beta * q, then the listed entries once more with p subtracted.  STEP: both.
-template <class T, int MODE>
-__global__ void __launch_bounds__(DISTILL_THREADS) k_distill(const DistillArgs g) {
-    __shared__ Listed L;
+// A warp's part of the share's sum: with the maximum of its logits first.
+template <class T>
+__device__ __noinline__ Partial sum_carefully(const Share<T>& s, float b2) {
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    const float weight = g.weight ? g.weight[row] : 1.0f;
-    const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
-    T* grad = MODE == LOSS ? nullptr : static_cast<T*>(g.grad) + row * g.grad_pitch;
-    bool live = weight != 0.0f;
-    if (live) {
-        list_teacher<T>(L, g, row, logits);
-        live = L.any != 0;
+    float high = -INFINITY, other = -INFINITY;
+    for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) larger_16<T>(high, other, s.piece(i));
+    high = fmaxf(upper<T>(high), other);
+    if (s.head + tid < s.first) high = fmaxf(high, to_float(s.row[s.head + tid]));
+    if (s.tail + tid < s.stop) high = fmaxf(high, to_float(s.row[s.tail + tid]));
+    high = warp_max(high);
+    const float low = high == -INFINITY ? 0.0f : high;
+    const bool far = is_far(low * b2);
+    auto weight = [&](float l) { return far ? far_weight(l, low) : exp2_fast(fmaf(l, b2, -low * b2)); };
+    float sum = 0.0f;
+    for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) {
+        float v[VEC<T>];
+        unpack_16<T>(s.piece(i), v);
+#pragma unroll
+        for (int j = 0; j < VEC<T>; ++j) sum += weight(v[j]);
     }
-    if (!live) {  // padding: nothing of the row is read
-        if (MODE != LOSS) for (int32_t k = tid; k < g.cols; k += DISTILL_THREADS) grad[k] = from_float<T>(0.0f);
-        if (tid == 0 && MODE != GRAD) g.loss[row] = 0.0f;
-        if (tid == 0 && MODE == LOSS) g.lse_out[row] = 0.0f;
+    if (s.head + tid < s.first) sum += weight(to_float(s.row[s.head + tid]));
+    if (s.tail + tid < s.stop) sum += weight(to_float(s.row[s.tail + tid]));
+    return Partial{high, warp_total(sum)};
+}
+template <class T>
+__device__ __forceinline__ Partial sum_of(const Share<T>& s, float b2) {
+    constexpr int V = VEC<T>, AT_ONCE = 4;
+    const int tid = threadIdx.x;
+    // The reference is the largest of the warp's first pieces, which spares a pass for the maximum: sums are good as long as they
+    // stay below 2^100, and what does not is done over with the maximum.
+    float2 sums = both(0.0f), more = both(0.0f);
+    float ref = -INFINITY, other = -INFINITY;
+    if (tid < s.pieces) larger_16<T>(ref, other, s.piece(tid));
+    ref = warp_max(fmaxf(upper<T>(ref), other));
+    const float2 scale = both(b2), shift = both(-ref * b2);
+    auto add = [&](const uint4& raw) {
+        float v[V];
+        unpack_16<T>(raw, v);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const float2 a = fma_2(make_float2(v[j], v[j + 1]), scale, shift), b = fma_2(make_float2(v[j + 2], v[j + 3]), scale, shift);
+            sums = add_2(sums, make_float2(exp2_fast(a.x), exp2_fast(a.y)));
+            more = add_2(more, make_float2(exp2_fast(b.x), exp2_fast(b.y)));
+        }
+    };
+    int32_t i = tid;
+    for (; i + (AT_ONCE - 1) * SOFTMAX_THREADS < s.pieces; i += AT_ONCE * SOFTMAX_THREADS) {
+        uint4 raw[AT_ONCE];
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) raw[t] = s.piece(i + t * SOFTMAX_THREADS);
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) add(raw[t]);
+    }
+    for (; i < s.pieces; i += SOFTMAX_THREADS) add(s.piece(i));
+    float sum = (sums.x + sums.y) + (more.x + more.y);
+    if (s.head + tid < s.first) sum += exp2_fast(fmaf(to_float(s.row[s.head + tid]), b2, shift.x));
+    if (s.tail + tid < s.stop) sum += exp2_fast(fmaf(to_float(s.row[s.tail + tid]), b2, shift.x));
+    sum = warp_total(sum);
+    if (!(sum < 0x1p100f) || is_far(ref * b2)) return sum_carefully(s, b2);
+    return Partial{ref, sum};
+}
+
+// The row's largest logit and the number of categories that share it, by every warp for itself (far rows of which only lse is
+// known).
+template <class T>
+__device__ __noinline__ Partial count_largest(const T* logits, int32_t cols) {
+    const int lane = threadIdx.x & 31;
+    float high = -INFINITY, n = 0.0f;
+    for (int32_t k = lane; k < cols; k += 32) high = fmaxf(high, to_float(logits[k]));
+    high = warp_max(high);
+    for (int32_t k = lane; k < cols; k += 32) n += far_weight(to_float(logits[k]), high);
+    return Partial{high, warp_total(n)};
+}
+
+// q of a row, from the joined parts of its sum or from its lse.
+struct Softmax {
+    float ref, sum2;  // a logit, and log2 of the sum relative to it
+    float shift, each;
+    bool far, empty;
+    __device__ __forceinline__ static Softmax of(Partial p, float b2) {
+        Softmax s;
+        s.ref = p.ref;
+        s.far = is_far(p.ref * b2);
+        s.empty = p.ref == -INFINITY && p.sum == 0.0f;
+        s.sum2 = p.sum == INFINITY || (p.ref == -INFINITY && p.sum != 0.0f) ? NAN : log2f(p.sum);
+        if (!s.far) s.sum2 += fmaf(-p.ref, b2, __fmul_rn(p.ref, b2));  // relative to b2 ref itself
+        s.finish(b2);
+        return s;
+    }
+    __device__ __forceinline__ static Softmax of(float ref, float sum2, float b2) {
+        Softmax s;
+        s.ref = ref, s.sum2 = sum2;
+        s.far = is_far(ref * b2);
+        s.empty = ref == -INFINITY && sum2 == -INFINITY;
+        s.finish(b2);
+        return s;
+    }
+    template <class T>
+    __device__ __forceinline__ static Softmax of(float lse, const T* logits, int32_t cols, float b2) {
+        if (lse == lse && is_far(lse)) return of(count_largest(logits, cols), b2);  // so far out lse cannot say how many share the weight
+        return of(0.0f, lse * LOG2E, b2);
+    }
+    __device__ __forceinline__ void finish(float b2) {
+        each = far ? exp2_fast(-sum2) : 0.0f;
+        shift = fmaf(-ref, b2, -sum2);
+    }
+    __device__ __forceinline__ float q(float l, float b2) const { return empty ? 0.0f : far ? far_weight(l, ref) * each : exp2_fast(fmaf(l, b2, shift)); }
+};
+
+// The rows' sums (reference into loss, log2 of the sum into lse_out, from where k_listed takes them), and weight * beta * q into
+// grad.
+template <class T, int MODE>
+__global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_constant__ DistillArgs g) {
+    constexpr int V = VEC<T>, AT_ONCE = 4;
+    __shared__ Partial warps[SOFTMAX_THREADS / 32], ctas[8];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int64_t row = g.per_row == 1 ? blockIdx.x : blockIdx.x / g.per_row;
+    const int32_t part = static_cast<int32_t>(blockIdx.x - row * g.per_row);
+    const bool joined = MODE != GRAD && g.per_row > 1;  // the CTAs of a row form a cluster
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (joined) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const float weight = g.weight ? g.weight[row] : 1.0f;  // 0: padding, nothing of the row is read
+    const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
+    const Share<T> s(logits, g.cols, part * g.share, g.share);
+    const float b2 = g.beta * LOG2E;
+    Softmax soft{};
+    if (MODE == GRAD) {
+        if (weight != 0.0f) soft = Softmax::of(g.lse_in[row], logits, g.cols, b2);
+    } else {
+        Partial p{-INFINITY, 0.0f};
+        if (weight != 0.0f) p = sum_of(s, b2);
+        if (lane == 0) warps[tid >> 5] = p;
+        __syncthreads();
+        p = warps[lane & (SOFTMAX_THREADS / 32 - 1)];
+        for (int d = SOFTMAX_THREADS / 64; d; d >>= 1) p.join(Partial{__shfl_xor_sync(0xffffffffu, p.ref, d), __shfl_xor_sync(0xffffffffu, p.sum, d)}, b2);
+        p = Partial{__shfl_sync(0xffffffffu, p.ref, 0), __shfl_sync(0xffffffffu, p.sum, 0)};
+        if (joined) {
+            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row has started
+            if (tid < g.per_row) {
+                const uint32_t to = dense::peer_addr(dense::smem_u32(&ctas[part]), tid);
+                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(p.ref), "f"(p.sum) : "memory");
+            }
+            dense::cluster_sync_all();
+            p = ctas[0];
+            for (int c = 1; c < g.per_row; ++c) p.join(ctas[c], b2);
+        }
+        soft = Softmax::of(p, b2);
+        if (part == 0 && tid == 0) g.loss[row] = soft.ref, g.lse_out[row] = soft.sum2;
+    }
+    if (MODE == LOSS) return;
+    T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
+    const float scale = weight * g.beta;
+    const bool zeros = weight == 0.0f;
+    auto value = [&](float l) { return scale * soft.q(l, b2); };
+    if (tid < s.first - s.head) grad[s.head + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.head + tid])));
+    if (tid < s.stop - s.tail) grad[s.tail + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.tail + tid])));
+    if (((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15u) || soft.far) {
+        for (int32_t k = s.first + tid; k < s.tail; k += SOFTMAX_THREADS) grad[k] = from_float<T>(zeros ? 0.0f : value(to_float(logits[k])));
         return;
     }
-    float lse;
-    if (MODE == GRAD) {
-        lse = g.lse_in[row];
-    } else {
-        float most = -INFINITY;
-        for_row<T>(logits, g.cols, tid, DISTILL_THREADS, [&](int32_t, const float* v, auto cnt) {
-#pragma unroll
-            for (int j = 0; j < decltype(cnt)::value; ++j) most = v[j] > most || v[j] != v[j] ? v[j] : most;  // a NaN stays
-        });
-        most = most != most ? INFINITY : most;
-        most = g.beta * block_reduce<MaxOp>(most, L.scratch);
-        float total = 0.0f;
-        for_row<T>(logits, g.cols, tid, DISTILL_THREADS, [&](int32_t, const float* v, auto cnt) {
-#pragma unroll
-            for (int j = 0; j < decltype(cnt)::value; ++j) total += most == -INFINITY ? 0.0f : expf(g.beta * v[j] - most);
-        });
-        total = block_reduce<SumOp>(total, L.scratch);
-        lse = most == -INFINITY ? -INFINITY : most + logf(total);
-        float loss = 0.0f;
-        for (int j = tid; j < g.top; j += DISTILL_THREADS)
-            if (L.p[j] > 0.0f || L.p[j] != L.p[j]) loss += lse == -INFINITY ? INFINITY : L.p[j] * (logf(L.p[j]) - (L.z[j] - lse));
-        loss = block_reduce<SumOp>(loss, L.scratch);
-        if (tid == 0) g.loss[row] = loss;
-        if (tid == 0 && MODE == LOSS) g.lse_out[row] = lse;
+    uint4* out = reinterpret_cast<uint4*>(grad + s.first);
+    if (zeros) {
+        for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
+        return;
     }
-    if (MODE != LOSS) {
-        const float scale = weight * g.beta;
-        for_row<T>(logits, g.cols, tid, DISTILL_THREADS, [&](int32_t i, const float* v, auto cnt) {
-            constexpr int N = decltype(cnt)::value;
-            float x[N];
+    auto gradient = [&](const uint4& raw) {
+        float x[V];
+        unpack_16<T>(raw, x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = lse == -INFINITY ? 0.0f : scale * expf(g.beta * v[j] - lse);
-            store_n<T>(grad + i, x, cnt);
-        });
-        __syncthreads();  // the listed entries are written once more
-        for (int j = tid; j < g.top; j += DISTILL_THREADS) {
-            if (L.id[j] < 0) continue;
-            float p = 0.0f;
-            bool first = true;
-            for (int i = 0; i < g.top; ++i) {
-                if (L.id[i] != L.id[j]) continue;
-                if (i < j) first = false;
-                p += L.p[i];
-            }
-            if (first) grad[L.id[j]] = from_float<T>(scale * ((lse == -INFINITY ? 0.0f : expf(L.z[j] - lse)) - p));
+        for (int j = 0; j < V; j += 2) {
+            const float2 a = fma_2(make_float2(x[j], x[j + 1]), both(b2), both(soft.shift));
+            const float2 y = mul_2(make_float2(exp2_fast(a.x), exp2_fast(a.y)), both(scale));
+            x[j] = y.x, x[j + 1] = y.y;
+        }
+        return pack_16<T>(x);
+    };
+    int32_t i = tid;
+    for (; i + (AT_ONCE - 1) * SOFTMAX_THREADS < s.pieces; i += AT_ONCE * SOFTMAX_THREADS) {
+        uint4 raw[AT_ONCE];
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) raw[t] = s.piece(i + t * SOFTMAX_THREADS);
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) __stcs(out + i + t * SOFTMAX_THREADS, gradient(raw[t]));
+    }
+    for (; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, gradient(s.piece(i)));
+}
+
+// The lists: a team of one warp per row, or of all LIST_WARPS where lists are long.  Reads lse, writes the loss, and writes the
+// gradient's listed entries once more, with p subtracted before the rounding.
+template <class T, int MODE>
+__global__ void __launch_bounds__(32 * LIST_WARPS) k_listed(const __grid_constant__ DistillArgs g, int32_t teams) {
+    extern __shared__ int4 listed_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int team = teams == 1 ? 0 : warp, members = teams == 1 ? blockDim.x : 32, me = teams == 1 ? threadIdx.x : lane;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team;
+    const bool here = row < g.rows;
+    auto meet = [&] {
+        if (teams == 1) __syncthreads();
+        else __syncwarp();
+    };
+    const int top4 = (g.top + 3) & ~3;
+    int32_t* id = reinterpret_cast<int32_t*>(listed_smem) + 3 * top4 * team;  // -1 = not listed, up to a multiple of four
+    float* p = reinterpret_cast<float*>(id + top4);                           // beta * teacher, then the softmax over the listed
+    float* z = p + top4;                                                      // the student's logits there
+    const float weight = !here ? 0.0f : g.weight ? g.weight[row] : 1.0f;
+    const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
+    const float b2 = g.beta * LOG2E;
+    if (weight != 0.0f) {
+        if (me < top4 - g.top) id[g.top + me] = -1;
+#pragma unroll 4
+        for (int j = me; j < g.top; j += members) {
+            const int64_t k = load_as_int(g.ids, g.ids_type, row * g.ids_pitch + j);
+            const float t = g.beta * load_as_float(g.teacher, g.teacher_type, row * g.teacher_pitch + j);
+            const bool listed = k >= 0 && k < g.cols && !(t == -INFINITY);
+            id[j] = listed ? static_cast<int32_t>(k) : -1;
+            p[j] = t;
+            if (listed) z[j] = to_float(logits[k]);
         }
     }
+    meet();
+    bool some = false;
+    float most = -INFINITY, total = 0.0f;
+    if (weight != 0.0f) {
+        for (int j = lane; j < g.top; j += 32)
+            if (id[j] >= 0) {
+                most = fmaxf(most, p[j]);
+                some = true;
+            }
+        some = __any_sync(0xffffffffu, some);
+        most = warp_max(most);
+        for (int j = lane; j < g.top; j += 32) total += id[j] >= 0 ? expf(p[j] - most) : 0.0f;  // each warp of a team the same sum
+        total = warp_total(total);
+    }
+    meet();
+    if (weight != 0.0f)
+        for (int j = me; j < g.top; j += members) p[j] = id[j] >= 0 ? expf(p[j] - most) / total : 0.0f;
+    meet();
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' sums and gradients
+    if (!here) return;
+    const bool counts = weight != 0.0f && some;
+    if (!counts) {
+        if (MODE != GRAD && me == 0) g.loss[row] = 0.0f;
+        if (MODE != GRAD && me == 0) g.lse_out[row] = 0.0f;
+        if (MODE != LOSS && weight != 0.0f) {
+            T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
+            for (int32_t k = me; k < g.cols; k += members) grad[k] = from_float<T>(0.0f);
+        }
+        return;
+    }
+    const Softmax soft = MODE == GRAD ? Softmax::of(g.lse_in[row], logits, g.cols, b2) : Softmax::of(g.loss[row], g.lse_out[row], b2);
+    if (MODE != GRAD) {
+        meet();  // every thread has read the row's sum before the loss takes its place
+        if (teams > 1 || warp == 0) {
+            const float log_sum = soft.sum2 * LN2;
+            float loss = 0.0f;
+            for (int j = lane; j < g.top; j += 32)
+                if (id[j] >= 0 && !(p[j] == 0.0f)) loss += soft.empty ? INFINITY : p[j] * (logf(p[j]) - g.beta * (z[j] - soft.ref) + log_sum);
+            loss = warp_total(loss);
+            if (lane == 0) g.loss[row] = loss;
+            if (lane == 0) g.lse_out[row] = soft.empty ? -INFINITY : fmaf(g.beta, soft.ref, log_sum);
+        }
+    }
+    if (MODE != LOSS) {
+        T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
+        for (int j = me; j < g.top; j += members) {
+            const int32_t k = id[j];
+            if (k < 0) continue;
+            // the first entry of a category that is listed more than once writes for all of them
+            int same = 0;
+#pragma unroll 4
+            for (int i = 0; i < g.top; i += 4) {
+                const int4 o = *reinterpret_cast<const int4*>(id + i);
+                same += (o.x == k) + (o.y == k) + (o.z == k) + (o.w == k);
+            }
+            float share = p[j];
+            bool first = true;
+            if (same > 1) {
+                share = 0.0f;
+                for (int i = 0; i < g.top; ++i)
+                    if (id[i] == k) {
+                        first &= i >= j;
+                        share += p[i];
+                    }
+            }
+            if (first) grad[k] = from_float<T>(weight * g.beta * (soft.q(z[j], b2) - share));
+        }
+    }
+}
+
+// Positions of a row, counted from the last 16-byte boundary at or before it (the most that any row has).
+template <class T>
+int64_t positions(const void* p, int64_t pitch, int64_t cols) {
+    return aligned_to(p, 16) && pitch % VEC<T> == 0 ? cols : cols + VEC<T> - 1;
 }
 
 int32_t check_rows(const char* what, int64_t rows, int64_t cols, const void* p, int32_t type, int64_t pitch) {
@@ -308,11 +870,43 @@ int32_t check_rows(const char* what, int64_t rows, int64_t cols, const void* p, 
     return THRML_OK;
 }
 
-int32_t distill(thrml_ctx* ctx, void* stream, int mode, int64_t rows, int32_t type, const DistillArgs& g) {
+template <class T, int MODE>
+int32_t launch_distill(thrml_ctx* ctx, cudaStream_t stream, DistillArgs g) {
+    // CTAs per row: one for each 64 KB, eight at most that have to join; with few rows more, so that the GPU is covered.
+    const int64_t span = positions<T>(g.logits, g.pitch, g.cols), held = SOFTMAX_BYTES / sizeof(T);
+    int64_t per_row = (span + held - 1) / held;
+    if (MODE != GRAD) per_row = std::min<int64_t>(per_row, 8);
+    while (per_row <= 4 && g.rows * per_row < 2 * ctx->sm_count && span / (2 * per_row) >= SOFTMAX_THREADS * VEC<T>) per_row *= 2;
+    if (g.rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
+    g.per_row = static_cast<int32_t>(per_row);
+    g.share = static_cast<int32_t>(((span + per_row - 1) / per_row + VEC<T> - 1) / VEC<T> * VEC<T>);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    cfg.gridDim = dim3(static_cast<unsigned>(g.rows * per_row));
+    cfg.blockDim = dim3(SOFTMAX_THREADS);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {static_cast<unsigned>(per_row), 1, 1};
+    cfg.numAttrs = MODE != GRAD && per_row > 1 ? 1 : 0;
+    CU_TRY(cudaLaunchKernelEx(&cfg, k_softmax<T, MODE>, g));
+    // The lists start while the last rows are still at work; what they need of those they wait for.
+    const int32_t teams = g.top <= 128 ? LIST_WARPS : 1;
+    cfg.gridDim = dim3(static_cast<unsigned>((g.rows + teams - 1) / teams));
+    cfg.blockDim = dim3(32 * LIST_WARPS);
+    cfg.dynamicSmemBytes = 12 * static_cast<size_t>((g.top + 3) / 4 * 4) * teams;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    CU_TRY(cudaLaunchKernelEx(&cfg, k_listed<T, MODE>, g, teams));
+    return THRML_OK;
+}
+
+int32_t distill(thrml_ctx* ctx, void* stream, int mode, int64_t rows, int32_t type, DistillArgs g) {
     if (int32_t rc = check_rows("logits", rows, g.cols, g.logits, type, g.pitch)) return rc;
     if (mode != LOSS) {
         if (int32_t rc = check_rows("grad", rows, g.cols, g.grad, type, g.grad_pitch)) return rc;
-        if (g.grad == g.logits && g.grad_pitch != g.pitch) return fail(THRML_ERR_INVALID_ARG, "grad over the logits needs their pitch");
+        if (rows && g.grad == g.logits) return fail(THRML_ERR_INVALID_ARG, "grad must not be the logits themselves");
     }
     if (g.top < 0 || g.top > TOP_MAX) return fail(THRML_ERR_INVALID_ARG, "top is not within 0 and 1024");
     if (!is_index_type(g.ids_type)) return fail(THRML_ERR_INVALID_ARG, "ids: the element type is not an index type");
@@ -321,13 +915,12 @@ int32_t distill(thrml_ctx* ctx, void* stream, int mode, int64_t rows, int32_t ty
     if (!(g.beta > 0.0f) || g.beta == INFINITY) return fail(THRML_ERR_INVALID_ARG, "beta has to be positive and finite");
     if (rows == 0) return THRML_OK;
     if (g.top && (!g.ids || !g.teacher)) return fail(THRML_ERR_INVALID_ARG, "ids, teacher: null pointer");
-    if ((mode != GRAD && !g.loss) || (mode == LOSS && !g.lse_out) || (mode == GRAD && !g.lse_in)) return fail(THRML_ERR_INVALID_ARG, "loss, lse: null pointer");
+    if ((mode != GRAD && !g.loss) || (mode != GRAD && !g.lse_out) || (mode == GRAD && !g.lse_in)) return fail(THRML_ERR_INVALID_ARG, "loss, lse: null pointer");
+    g.rows = rows;
     return for_type(type, [&](auto e) {
         using T = decltype(e);
-        const auto kernel = mode == LOSS ? k_distill<T, LOSS> : mode == GRAD ? k_distill<T, GRAD> : k_distill<T, STEP>;
-        kernel<<<static_cast<unsigned>(rows), DISTILL_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(g);
-        CU_TRY(cudaGetLastError());
-        return THRML_OK;
+        const auto st = static_cast<cudaStream_t>(stream);
+        return mode == LOSS ? launch_distill<T, LOSS>(ctx, st, g) : mode == GRAD ? launch_distill<T, GRAD>(ctx, st, g) : launch_distill<T, STEP>(ctx, st, g);
     });
 }
 
@@ -365,13 +958,21 @@ int32_t thrml_adjust_logits(thrml_ctx* ctx, void* stream, int64_t rows, int64_t 
         if (rules->bias_ids && (!rules->bias_ptr || !rules->bias_values)) return fail(THRML_ERR_INVALID_ARG, "bias_ids without bias_ptr and bias_values");
         if (rules->mask && (rules->n_masks < 1 || rules->mask_pitch < (cols + 31) / 32)) return fail(THRML_ERR_INVALID_ARG, "mask: no masks, or a pitch smaller than a row's bits");
         if (rows == 0) return THRML_OK;
-        AdjustArgs g{logits, out, pitch, out_pitch, static_cast<int32_t>(cols), static_cast<int32_t>((cols + ADJUST_SLICE - 1) / ADJUST_SLICE), *rules};
-        if (rows * g.slices > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
-        const size_t smem = sizeof(uint32_t) * ADJUST_SLICE * ((rules->history ? 1 : 0) + (rules->bias_ids ? 1 : 0));
         return for_type(type, [&](auto e) {
             using T = decltype(e);
-            CU_TRY(cudaFuncSetAttribute(k_adjust<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * sizeof(uint32_t) * ADJUST_SLICE));
-            k_adjust<T><<<static_cast<unsigned>(rows * g.slices), ADJUST_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(g);
+            // As many CTAs as hold the row; with few rows, up to eight times as many, so that the GPU is covered.
+            const int64_t span = positions<T>(logits, pitch, cols);
+            int64_t per_row = (span + ADJUST_SHARE<T> - 1) / ADJUST_SHARE<T>;
+            const int64_t most = 8 * per_row;
+            while (2 * per_row <= most && rows * per_row < 2 * ctx->sm_count && span / (2 * per_row) >= 256) per_row *= 2;
+            const int64_t share = ((span + per_row - 1) / per_row + 63) / 64 * 64;
+            if (rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
+            // half of a full share's positions at a time (long histories) take 4 bytes each, the whole share 2
+            const int64_t count_bytes = std::max<int64_t>(2 * share, 4 * std::min<int64_t>(share, ADJUST_SHARE<T> / 2));
+            const AdjustArgs g{logits, out, pitch, out_pitch, static_cast<int32_t>(cols), static_cast<int32_t>(share), static_cast<int32_t>(per_row), static_cast<int32_t>(count_bytes / 4), *rules};
+            const size_t smem = 16 * ADJUST_PIECES * ADJUST_THREADS + (rules->history ? count_bytes : 0) + (rules->bias_ids ? share / 8 : 0);
+            CU_TRY(cudaFuncSetAttribute(k_adjust<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * ADJUST_PIECES * ADJUST_THREADS + ADJUST_SHARE<T> * 2 + ADJUST_SHARE<T> / 8));
+            k_adjust<T><<<static_cast<unsigned>(rows * per_row), ADJUST_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(g);
             CU_TRY(cudaGetLastError());
             return THRML_OK;
         });
@@ -387,10 +988,25 @@ int32_t thrml_draw_categories(thrml_ctx* ctx, void* stream, int64_t rows, int64_
         if (row_offset < 0 || row_offset > (int64_t{1} << 32) - rows) return fail(THRML_ERR_INVALID_ARG, "row_offset is out of range");
         if (rows == 0) return THRML_OK;
         if (!out) return fail(THRML_ERR_INVALID_ARG, "out: null pointer");
-        const DrawArgs g{logits, beta, noise, out, pitch, noise_pitch, static_cast<int32_t>(cols), static_cast<uint32_t>(row_offset), make_round_keys(key)};
+        // A CTA per row, or a cluster of up to eight where there are few rows for the GPU.
+        int64_t per_row = 1;
+        while (per_row < 8 && rows * per_row < 4 * ctx->sm_count && cols / (2 * per_row) >= DRAW_THREADS * DRAW_GROUP) per_row *= 2;
+        const int64_t share = ((cols + per_row - 1) / per_row + DRAW_GROUP - 1) / DRAW_GROUP * DRAW_GROUP;
+        if (rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
+        const DrawArgs g{logits, beta, noise, out, pitch, noise_pitch, static_cast<int32_t>(cols), static_cast<int32_t>(share), static_cast<int32_t>(per_row),
+                         static_cast<uint32_t>(row_offset), make_round_keys(key)};
         return for_type(type, [&](auto e) {
-            k_draw<decltype(e)><<<static_cast<unsigned>(rows), DRAW_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(g);
-            CU_TRY(cudaGetLastError());
+            using T = decltype(e);
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(static_cast<unsigned>(rows * per_row));
+            cfg.blockDim = dim3(DRAW_THREADS);
+            cfg.stream = static_cast<cudaStream_t>(stream);
+            cudaLaunchAttribute cluster;
+            cluster.id = cudaLaunchAttributeClusterDimension;
+            cluster.val.clusterDim = {static_cast<unsigned>(per_row), 1, 1};
+            cfg.attrs = &cluster;
+            cfg.numAttrs = per_row > 1 ? 1 : 0;
+            CU_TRY(cudaLaunchKernelEx(&cfg, noise ? k_draw<T, true> : k_draw<T, false>, g));
             return THRML_OK;
         });
     });
@@ -421,10 +1037,11 @@ int32_t thrml_distill_grad(thrml_ctx* ctx, void* stream, int64_t rows, int64_t c
 
 int32_t thrml_distill_step(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, int64_t top, const void* ids,
                            int32_t ids_type, int64_t ids_pitch, const void* teacher, int32_t teacher_type, int64_t teacher_pitch, float beta, const float* weight,
-                           float* loss, void* grad, int64_t grad_pitch) {
+                           float* loss, float* lse, void* grad, int64_t grad_pitch) {
     return guarded(ctx, [&] {
         DistillArgs g = distill_args(logits, pitch, cols, top, ids, ids_type, ids_pitch, teacher, teacher_type, teacher_pitch, beta, weight);
         g.loss = loss;
+        g.lse_out = lse;
         g.grad = grad;
         g.grad_pitch = grad_pitch;
         return distill(ctx, stream, STEP, rows, type, g);

@@ -284,19 +284,19 @@ def distill_loss(logits, ids, teacher, *, beta=1.0, weight=None):
 
 def distill_grad(logits, lse, ids, teacher, *, beta=1.0, weight=None, out=None):
     """The gradient of sum_r weight[r] * loss[r] by the logits, in their type, from `distill_loss`'s lse: weight (f32 per row, None = 1)
-    is what comes from above.  `out` may be `logits` itself."""
+    is what comes from above."""
     a = _distill_args(logits, ids, teacher, beta, weight)
-    out, pitch = (logits, a[6]) if out is logits else _new_or(out, "out", *logits.shape, logits.dtype, logits.device)[::2]
+    out, _, pitch = _new_or(out, "out", *logits.shape, logits.dtype, logits.device)
     lse_ptr = _vector(lse, "lse", logits.device, torch.float32, logits.shape[0])
     _check(lib().thrml_distill_grad(*a, lse_ptr, out.data_ptr(), pitch))
     return out
 
 
 def distill_step(logits, ids, teacher, *, beta=1.0, weight=None, out=None):
-    """(loss, gradient) in one call: `distill_loss` and `distill_grad` for weights that are known beforehand.  `out` (the gradient) may be
-    `logits` itself."""
+    """(loss, gradient) in one call: `distill_loss` and `distill_grad` for weights that are known beforehand.  `out`: the
+    gradient."""
     a = _distill_args(logits, ids, teacher, beta, weight)
-    out, pitch = (logits, a[6]) if out is logits else _new_or(out, "out", *logits.shape, logits.dtype, logits.device)[::2]
-    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-    _check(lib().thrml_distill_step(*a, loss.data_ptr(), out.data_ptr(), pitch))
-    return loss, out
+    out, _, pitch = _new_or(out, "out", *logits.shape, logits.dtype, logits.device)
+    loss = torch.empty((2, logits.shape[0]), dtype=torch.float32, device=logits.device)  # and lse
+    _check(lib().thrml_distill_step(*a, loss.data_ptr(), loss.data_ptr() + 4 * logits.shape[0], out.data_ptr(), pitch))
+    return loss[0], out
