@@ -261,10 +261,11 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
 // hardware exponential and no logarithm, and nearly every category fails it.  The ones that pass get their score in f64
 // (where two scores that f32 cannot tell apart have an order), which decides.  B starts from approximate scores of each
 // thread's first categories, lowered by more than their error, and rises with the scores found, shared in the CTA.
-// Bound by instruction issue: ten rounds of the generator serve four categories.
+// Bound by instruction issue: ten rounds of the generator serve four categories.  256 x 131072 bf16: 52 us with two CTAs a
+// row, 60 with four and 75 with eight, whose starts and first, loose bounds cost more than they spread.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int DRAW_THREADS = 256, DRAW_GROUP = 8;  // categories of a thread's turn: two generator calls
-constexpr int DRAW_AHEAD = 4;                      // turns whose logits are on their way
+constexpr int DRAW_THREADS = 256, DRAW_GROUP = 8;  // categories that share two generator calls
+constexpr int DRAW_AT_ONCE = 2;                     // groups of a thread whose logits are in flight together
 
 struct DrawArgs {
     const void* logits;
@@ -289,6 +290,12 @@ struct Best {
     }
 };
 
+// -log(-log u) to well within 1e-3, for u in (0, 1); near 1 the inner logarithm is a series in 1 - u.
+__device__ __forceinline__ float gumbel_fast(float u) {
+    const float rest = 1.0f - u, t = rest < 0.125f ? rest * fmaf(rest, fmaf(rest, 0.33333333f, 0.5f), 1.0f) : -__logf(u);
+    return -__logf(t);
+}
+
 // The scores in f64 of those of DRAW_GROUP categories that reach the bound, out of line: few turns have any.
 template <class T>
 __device__ __noinline__ void weigh(Best& best, int32_t* bound, const DrawArgs& g, const T* logits, const float* noise, float beta, int64_t row, int32_t k, int32_t to) {
@@ -302,7 +309,7 @@ __device__ __noinline__ void weigh(Best& best, int32_t* bound, const DrawArgs& g
             if (beta != INFINITY) {
                 const float u = noise ? noise[k + j] : u23_open(pick(w, j - h));
                 const float b = from_ordered(*static_cast<volatile int32_t*>(bound));
-                if (fmaf(beta, l, -__logf(1.0f - u)) + 1e-2f + 1e-5f * (fabsf(beta * l) + fabsf(b)) < b) continue;  // -ln u >= 1 - u, once more for each
+                if (beta * l + gumbel_fast(u) + (1e-2f + 1e-5f * fabsf(beta * l)) < b) continue;
                 score = __dsub_rn(__dmul_rn(beta, l), log(-log(static_cast<double>(u))));
             }
             best.take(score, k + j);
@@ -312,12 +319,12 @@ __device__ __noinline__ void weigh(Best& best, int32_t* bound, const DrawArgs& g
 }
 
 template <class T, bool GIVEN>
-__global__ void __launch_bounds__(DRAW_THREADS, 5) k_draw(const __grid_constant__ DrawArgs g) {
+__global__ void __launch_bounds__(DRAW_THREADS, 4) k_draw(const __grid_constant__ DrawArgs g) {
     __shared__ Best warps[DRAW_THREADS / 32], ctas[8];
     __shared__ int32_t bound;
     const int tid = threadIdx.x, lane = tid & 31;
-    const int64_t row = blockIdx.x / g.per_row;
-    const int32_t part = static_cast<int32_t>(blockIdx.x % g.per_row), from = part * g.share, to = min(g.cols, from + g.share);
+    const int64_t row = g.per_row == 1 ? blockIdx.x : blockIdx.x / g.per_row;
+    const int32_t part = static_cast<int32_t>(blockIdx.x - row * g.per_row), from = part * g.share, to = min(g.cols, from + g.share);
     if (g.per_row > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const float beta = g.beta ? g.beta[row] : 1.0f;
     const bool greedy = beta == INFINITY;
@@ -326,107 +333,113 @@ __global__ void __launch_bounds__(DRAW_THREADS, 5) k_draw(const __grid_constant_
     const bool wide = on_16(logits + from);  // shares are multiples of DRAW_GROUP
     const float b2 = beta * LOG2E;
 
-    // The logits of a turn, through shared memory, DRAW_AHEAD turns ahead; a thread reads what it asked for.  What lies behind the
-    // share is masked.
     constexpr int PIECES = DRAW_GROUP / VEC<T>;
-    __shared__ uint4 ring[DRAW_AHEAD][PIECES][DRAW_THREADS];
-    auto fetch = [&](int32_t k, int turn) {
-        uint4(*slot)[DRAW_THREADS] = ring[turn % DRAW_AHEAD];
-        if (k < to) {
-            if (wide && k + DRAW_GROUP <= to) {
+    struct Group {
+        uint4 raw[PIECES];
+    };
+    // The logits of a group as they lie in memory; what lies behind the share is masked.
+    auto load = [&](int32_t k) {
+        Group q;
+        if (wide && k + DRAW_GROUP <= to) {
 #pragma unroll
-                for (int h = 0; h < PIECES; ++h) copy_16_async(&slot[h][tid], logits + k + h * VEC<T>);
-            } else {
-                for (int h = 0; h < PIECES; ++h) {
-                    slot[h][tid] = nothing_16<T>();
-                    for (int j = 0; j < VEC<T>; ++j)
-                        if (k + h * VEC<T> + j < to) reinterpret_cast<T*>(&slot[h][tid])[j] = logits[k + h * VEC<T> + j];
-                }
+            for (int h = 0; h < PIECES; ++h) q.raw[h] = *reinterpret_cast<const uint4*>(logits + k + h * VEC<T>);
+        } else {
+#pragma unroll
+            for (int h = 0; h < PIECES; ++h) {
+                q.raw[h] = nothing_16<T>();
+#pragma unroll
+                for (int j = 0; j < VEC<T>; ++j)
+                    if (k + h * VEC<T> + j < to) reinterpret_cast<T*>(&q.raw[h])[j] = logits[k + h * VEC<T> + j];
             }
         }
-        commit_copies();
+        return q;
     };
-    auto logits_of = [&](int turn, float (&l)[DRAW_GROUP]) {
+    // Four uniforms.  From the key: 1 + n 2^-23, where u = (n + 1/2) 2^-23; given: u.
+    auto draw = [&](int32_t k, float (&f)[4]) {
+        if (GIVEN) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = k + j < to ? noise[k + j] : 0.0f;
+        } else {
+            const U4 w = philox4x32_10_rk(g.row_offset + static_cast<uint32_t>(row), 0u, static_cast<uint32_t>(k) >> 2, TAG_DRAW, g.rk);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(__funnelshift_r(pick(w, j), 0x7fu, 9));  // the exponent of 1, then n
+        }
+    };
+    // Whether any of a group can exceed the bound `b`.
+    auto reaches = [&](const Group& q, int32_t k, float b) {
+        bool some = false;
+        // c = the bound in base 2, lowered by the roundings of c and of beta l log2(e), 2^-22 of their sizes (a category 60 or
+        // more below c is out of reach of them), and by the exponential's error
+        const float c = b * LOG2E, low = b == INFINITY ? b : c - (fabsf(c) + 60.0f) * 0x1p-21f - 1e-5f;
+        float l[DRAW_GROUP];
 #pragma unroll
         for (int h = 0; h < PIECES; ++h) {
             float v[VEC<T>];
-            unpack_16<T>(ring[turn % DRAW_AHEAD][h][tid], v);
+            unpack_16<T>(q.raw[h], v);
 #pragma unroll
             for (int j = 0; j < VEC<T>; ++j) l[h * VEC<T> + j] = v[j];
         }
-    };
-    // Their uniforms.  From the key: 1 + n 2^-23, where u = (n + 1/2) 2^-23; given: u.
-    auto draw = [&](int32_t k, float (&f)[DRAW_GROUP]) {
-        if (greedy) return;
-        if (GIVEN) {
+        if (greedy) {
 #pragma unroll
-            for (int j = 0; j < DRAW_GROUP; ++j) f[j] = k + j < to ? noise[k + j] : 0.0f;
-        } else {
+            for (int j = 0; j < DRAW_GROUP; ++j) some |= l[j] >= b;
+            return some;
+        }
 #pragma unroll
-            for (int h = 0; h < DRAW_GROUP; h += 4) {
-                const U4 w = philox4x32_10_rk(g.row_offset + static_cast<uint32_t>(row), 0u, static_cast<uint32_t>(k + h) >> 2, TAG_DRAW, g.rk);
+        for (int h = 0; h < DRAW_GROUP; h += 4) {
+            float f[4];
+            draw(k + h, f);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) f[h + j] = __uint_as_float(__funnelshift_r(pick(w, j), 0x7fu, 9));  // the exponent of 1, then n
+            for (int j = 0; j < 4; j += 2) {
+                const float2 a = fma_2(make_float2(l[h + j], l[h + j + 1]), both(b2), both(-low)), e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+                // 1 - u = 2 - f - 2^-24 for the key's; the rounding of 2 - 2^-22 - e is covered.  What is no number passes here.
+                if (GIVEN) {
+                    some |= !(1.0f - f[j] > e.x) | !(1.0f - f[j + 1] > e.y);
+                } else {
+                    const float2 least = fma_2(e, both(-1.0f), both(2.0f - 0x1p-22f));
+                    some |= !(f[j] < least.x) | !(f[j + 1] < least.y);
+                }
             }
         }
+        return some;
     };
 
     Best best{0.0, -1};
     if (beta >= 0.0f) {
-        // A first bound, from each thread's first categories.
+        // A first bound, from each thread's first group.
         float first = -INFINITY;
         const int32_t k0 = from + tid * DRAW_GROUP, step = DRAW_THREADS * DRAW_GROUP;
-        for (int t = 0; t < DRAW_AHEAD; ++t) fetch(k0 + t * step, t);
-        wait_copies<DRAW_AHEAD - 1>();
         if (k0 < to) {
-            float l[DRAW_GROUP], f[DRAW_GROUP];
-            draw(k0, f);
-            logits_of(0, l);
+            const Group q = load(k0);
 #pragma unroll
-            for (int j = 0; j < (GIVEN ? DRAW_GROUP : 4); ++j) {
-                float s = l[j];
-                if (!greedy) {
-                    const float u = GIVEN ? f[j] : (f[j] - 1.0f) + 0x1p-24f;
-                    s = fmaf(beta, l[j], -__logf(-__logf(u)));
-                    s -= 1e-2f + 1e-5f * fabsf(s);
-                    if (!(u < 0.9f)) s = -INFINITY;  // up to there the two logarithms are good to 1e-2 by far
+            for (int h = 0; h < DRAW_GROUP; h += 4) {
+                float f[4];
+                if (!greedy) draw(k0 + h, f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float l = to_float(reinterpret_cast<const T*>(q.raw)[h + j]);
+                    float s = l;
+                    if (!greedy) {
+                        const float z = beta * l;
+                        s = z + gumbel_fast(GIVEN ? f[j] : (f[j] - 1.0f) + 0x1p-24f) - (1e-2f + 1e-5f * fabsf(z));
+                    }
+                    if (l > -INFINITY && s < INFINITY) first = fmaxf(first, s);
                 }
-                if (l[j] > -INFINITY && s < INFINITY) first = fmaxf(first, s);
             }
         }
-        for (int d = 16; d; d >>= 1) first = fmaxf(first, __shfl_xor_sync(0xffffffffu, first, d));
+        const int32_t highest = __reduce_max_sync(0xffffffffu, ordered(first));
         if (tid == 0) bound = ordered(-INFINITY);
         __syncthreads();
-        if (lane == 0) atomicMax(&bound, ordered(first));
+        if (lane == 0) atomicMax(&bound, highest);
         __syncthreads();
-        for (int32_t k = k0, turn = 0; k < to; k += step, ++turn) {
-            float l[DRAW_GROUP], f[DRAW_GROUP];
-            wait_copies<DRAW_AHEAD - 1>();
-            logits_of(turn, l);
-            fetch(k + DRAW_AHEAD * step, turn);  // into the place just read
-            const float b = from_ordered(*static_cast<volatile int32_t*>(&bound));
-            bool some = false;
-            if (greedy) {
+        for (int32_t k = k0; k < to; k += DRAW_AT_ONCE * step) {
+            Group q[DRAW_AT_ONCE];
 #pragma unroll
-                for (int j = 0; j < DRAW_GROUP; ++j) some |= l[j] >= b;
-            } else {
-                draw(k, f);
-                // c = the bound in base 2, lowered by the roundings of c and of beta l log2(e), 2^-22 of their sizes (a category 60 or
-                // more below c is out of reach of them), and by the exponential's error
-                const float c = b * LOG2E, low = b == INFINITY ? b : c - (fabsf(c) + 60.0f) * 0x1p-21f - 1e-5f;
+            for (int t = 0; t < DRAW_AT_ONCE; ++t)
+                if (k + t * step < to) q[t] = load(k + t * step);
 #pragma unroll
-                for (int j = 0; j < DRAW_GROUP; j += 2) {
-                    const float2 a = fma_2(make_float2(l[j], l[j + 1]), both(b2), both(-low)), e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
-                    // 1 - u = 2 - f - 2^-24 for the key's; the rounding of 2 - 2^-22 - e is covered.  What is no number passes here.
-                    if (GIVEN) {
-                        some |= !(1.0f - f[j] > e.x) | !(1.0f - f[j + 1] > e.y);
-                    } else {
-                        const float2 least = fma_2(e, both(-1.0f), both(2.0f - 0x1p-22f));
-                        some |= !(f[j] < least.x) | !(f[j + 1] < least.y);
-                    }
-                }
-            }
-            if (some) weigh<T>(best, &bound, g, logits, noise, beta, row, k, to);
+            for (int t = 0; t < DRAW_AT_ONCE; ++t)
+                if (k + t * step < to && reaches(q[t], k + t * step, from_ordered(*static_cast<volatile int32_t*>(&bound))))
+                    weigh<T>(best, &bound, g, logits, noise, beta, row, k + t * step, to);
         }
     }
     for (int d = 16; d; d >>= 1) {
@@ -990,7 +1003,7 @@ int32_t thrml_draw_categories(thrml_ctx* ctx, void* stream, int64_t rows, int64_
         if (!out) return fail(THRML_ERR_INVALID_ARG, "out: null pointer");
         // A CTA per row, or a cluster of up to eight where there are few rows for the GPU.
         int64_t per_row = 1;
-        while (per_row < 8 && rows * per_row < 4 * ctx->sm_count && cols / (2 * per_row) >= DRAW_THREADS * DRAW_GROUP) per_row *= 2;
+        while (per_row < 8 && rows * per_row < 2 * ctx->sm_count && cols / (2 * per_row) >= DRAW_THREADS * DRAW_GROUP) per_row *= 2;
         const int64_t share = ((cols + per_row - 1) / per_row + DRAW_GROUP - 1) / DRAW_GROUP * DRAW_GROUP;
         if (rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
         const DrawArgs g{logits, beta, noise, out, pitch, noise_pitch, static_cast<int32_t>(cols), static_cast<int32_t>(share), static_cast<int32_t>(per_row),
