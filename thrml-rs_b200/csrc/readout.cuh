@@ -77,37 +77,6 @@ __device__ __forceinline__ uint4 pack_16(const float* v) {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// n values of a row to dst (16 bytes at once where dst allows it).
-template <class T, int N>
-__device__ __forceinline__ void store_n(T* dst, const float* v, Count<N>) {
-    if (N == VEC<T> && on_16(dst)) {
-        *reinterpret_cast<uint4*>(dst) = pack_16<T>(v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) dst[i] = from_float<T>(v[i]);
-    }
-}
-// f(index, values, Count) over row[0 .. n): up to the first 16-byte boundary one by one, then 16 bytes at a time, then one by
-// one.  Thread `tid` of `threads` takes its share; every thread calls f for its own elements only.
-template <class T, class F>
-__device__ __forceinline__ void for_row(const T* row, int32_t n, int tid, int threads, F f) {
-    const int32_t ahead = min(n, static_cast<int32_t>((-reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T)));
-    const int32_t vecs = (n - ahead) / VEC<T>, behind = ahead + vecs * VEC<T>;
-    if (tid < ahead) {
-        const float v[1] = {to_float(row[tid])};
-        f(tid, v, Count<1>{});
-    }
-    for (int32_t i = tid; i < vecs; i += threads) {
-        float v[VEC<T>];
-        unpack_16<T>(*reinterpret_cast<const uint4*>(row + ahead + i * VEC<T>), v);
-        f(ahead + i * VEC<T>, v, Count<VEC<T>>{});
-    }
-    if (behind + tid < n) {
-        const float v[1] = {to_float(row[behind + tid])};
-        f(behind + tid, v, Count<1>{});
-    }
-}
-
 // Two f32 operations in one instruction.
 __device__ __forceinline__ float2 fma_2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -174,6 +143,23 @@ struct Pieces {
     }
     // Whether pieces of `to` lie on 16-byte boundaries as the row's do.
     __device__ __forceinline__ bool same_phase(const T* to) const { return ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(row)) & 15u) == 0; }
+};
+
+// One CTA's share of a row: whole pieces of 16 bytes from `first` on, and up to VEC - 1 elements before and behind them.
+template <class T>
+struct Share {
+    const T* row;
+    int32_t head, first, pieces, tail, stop;  // elements [head, first), pieces from first, elements [tail, stop)
+    __device__ __forceinline__ Share(const T* r, int32_t cols, int32_t from, int32_t share) : row(r) {
+        const Pieces<T> p(r, cols);
+        const int32_t to = min(p.end, from + share);
+        head = max(from - p.ahead, 0);
+        stop = max(to - p.ahead, head);
+        first = min(from < p.ahead ? from + VEC<T> - p.ahead : head, stop);
+        pieces = (stop - first) / VEC<T>;
+        tail = first + pieces * VEC<T>;
+    }
+    __device__ __forceinline__ uint4 piece(int32_t i) const { return *reinterpret_cast<const uint4*>(row + first + i * VEC<T>); }
 };
 
 // ---- host side

@@ -530,23 +530,6 @@ struct Partial {
     }
 };
 
-// One CTA's share of a row: whole pieces of 16 bytes from `first` on, and up to VEC - 1 elements before and behind them.
-template <class T>
-struct Share {
-    const T* row;
-    int32_t head, first, pieces, tail, stop;  // elements [head, first), pieces from first, elements [tail, stop)
-    __device__ __forceinline__ Share(const T* r, int32_t cols, int32_t from, int32_t share) : row(r) {
-        const Pieces<T> p(r, cols);
-        const int32_t to = min(p.end, from + share);
-        head = max(from - p.ahead, 0);
-        stop = max(to - p.ahead, head);
-        first = min(from < p.ahead ? from + VEC<T> - p.ahead : head, stop);
-        pieces = (stop - first) / VEC<T>;
-        tail = first + pieces * VEC<T>;
-    }
-    __device__ __forceinline__ uint4 piece(int32_t i) const { return *reinterpret_cast<const uint4*>(row + first + i * VEC<T>); }
-};
-
 // The larger of the even and of the odd elements of 16 bytes.  A bf16 in the upper half of a word is compared with the lower half
 // as further fraction bits, which do not change which is the largest; upper() drops them.  What is no number, or is made one by
 // those bits, gives way (an infinity that is missed so shows in the sum).

@@ -1,5 +1,7 @@
 // The readout's 8-bit product: activations quantised with one scale per token, weights with one scale per channel, the sum
 // of products exact in 32-bit integers on the tensor cores (tcgen05 kind::i8, accumulators in tensor memory).
+#include <algorithm>
+
 #include "readout.cuh"
 #include "tensor_core.cuh"
 
@@ -7,6 +9,9 @@ using namespace thrml;
 using namespace thrml::readout;
 
 namespace {
+
+template <int N>
+__device__ __forceinline__ bool aligned_for(const void* p) { return (reinterpret_cast<uintptr_t>(p) % N) == 0; }
 
 // ---------------------------------------------------------------------------------------------------------
 // Rows in 8 bits.
@@ -25,7 +30,9 @@ __device__ __forceinline__ int32_t quantise(float x, float scale, float inverse)
     return static_cast<int32_t>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
-constexpr int QUANT_THREADS = 256;
+// Bound by memory.  A CTA has a row: as many threads as hold it in four 16-byte pieces each (32 to 256; a longer row's rest is
+// read a second time), in registers between the maximum and the quotients.
+constexpr int QUANT_THREADS = 256, QUANT_PIECES = 4;
 
 struct QuantArgs {
     const void* x;
@@ -36,33 +43,82 @@ struct QuantArgs {
     int32_t cols;
 };
 
-// One CTA per row: the largest magnitude, then the row once more.
 template <class T>
-__global__ void __launch_bounds__(QUANT_THREADS) k_quantize(const QuantArgs g) {
+__global__ void __launch_bounds__(QUANT_THREADS) k_quantize(const __grid_constant__ QuantArgs g) {
+    constexpr int V = VEC<T>;
     __shared__ uint32_t sh[QUANT_THREADS / 32];
-    const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, threads = blockDim.x;
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(g.x) + row * g.x_pitch;
     int8_t* q = g.q + row * g.q_pitch;
-    uint32_t most = 0;  // the bits of |x| order as the magnitudes do, with infinity and then NaN above them
-    for_row<T>(x, g.cols, tid, QUANT_THREADS, [&](int32_t, const float* v, auto cnt) {
+    const Share<T> s(x, g.cols, 0, g.cols + V);
+    uint4 raw[QUANT_PIECES];
 #pragma unroll
-        for (int j = 0; j < decltype(cnt)::value; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-    });
+    for (int t = 0; t < QUANT_PIECES; ++t)
+        if (tid + t * threads < s.pieces) raw[t] = s.piece(tid + t * threads);
+    uint32_t most = 0;  // the bits of |x| order as the magnitudes do, with infinity and then NaN above them
+    auto look = [&](const uint4& r) {
+        float v[V];
+        unpack_16<T>(r, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    };
+    auto edge = [&](auto f) {
+        if (s.head + tid < s.first) f(s.head + tid);
+        if (s.tail + tid < s.stop) f(s.tail + tid);
+    };
+#pragma unroll
+    for (int t = 0; t < QUANT_PIECES; ++t)
+        if (tid + t * threads < s.pieces) look(raw[t]);
+    for (int32_t i = tid + QUANT_PIECES * threads; i < s.pieces; i += threads) look(s.piece(i));
+    edge([&](int32_t k) { most = max(most, __float_as_uint(to_float(x[k])) & 0x7fffffffu); });
     most = __reduce_max_sync(0xffffffffu, most);
     if ((tid & 31) == 0) sh[tid >> 5] = most;
     __syncthreads();
-    for (int w = 0; w < QUANT_THREADS / 32; ++w) most = max(most, sh[w]);
+    for (int w = 0; w < threads / 32; ++w) most = max(most, sh[w]);
     const float scale = __fdiv_rn(__uint_as_float(most), 127.0f);
     if (tid == 0) g.scale[row] = scale;
     const bool zeros = scale == 0.0f || !(scale < INFINITY);
     const float lift = scale < 0x1p-100f ? 0x1p100f : 1.0f;  // a power of two: exact, and the reciprocal stays finite
     const float lifted = scale * lift, inverse = 1.0f / lifted;
-    for_row<T>(x, g.cols, tid, QUANT_THREADS, [&](int32_t i, const float* v, auto cnt) {
-        constexpr int N = decltype(cnt)::value;
+    auto one = [&](float v) { return zeros ? 0 : quantise(v * lift, lifted, inverse); };
+    auto put = [&](int32_t i, const uint4& r) {
+        float v[V];
+        unpack_16<T>(r, v);
+        uint32_t w[V / 4];
+        bool near = zeros || lift != 1.0f;
 #pragma unroll
-        for (int j = 0; j < N; ++j) q[i + j] = static_cast<int8_t>(zeros ? 0 : quantise(v[j] * lift, lifted, inverse));
-    });
+        for (int j = 0; j < V; j += 4) {
+            uint32_t b[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                // adding 1.5 2^23 rounds to an integer, whose low byte is the sum's; a product next to a half is decided below
+                const float y = v[j + t] * inverse, sum = y + 0x1.8p23f;
+                near |= fabsf(y - (sum - 0x1.8p23f)) > 0.5f - 0x1p-12f;
+                b[t] = __float_as_uint(sum);
+            }
+            w[j / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        }
+        if (near) {
+#pragma unroll
+            for (int j = 0; j < V; j += 4)
+                w[j / 4] = (one(v[j]) & 0xff) | (one(v[j + 1]) & 0xff) << 8 | (one(v[j + 2]) & 0xff) << 16 | static_cast<uint32_t>(one(v[j + 3])) << 24;
+        }
+        int8_t* to = q + s.first + i * V;
+        if (aligned_for<V>(to)) {
+            if (V == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[V / 4 - 1]);
+            else *reinterpret_cast<uint32_t*>(to) = w[0];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) to[j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < QUANT_PIECES; ++t)
+        if (tid + t * threads < s.pieces) put(tid + t * threads, raw[t]);
+    for (int32_t i = tid + QUANT_PIECES * threads; i < s.pieces; i += threads) put(i, s.piece(i));
+    edge([&](int32_t k) { q[k] = static_cast<int8_t>(one(to_float(x[k]))); });
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -83,7 +139,7 @@ struct ProductArgs {
 };
 
 template <int BM>
-__host__ __device__ constexpr int prod_stages() { return BM <= 64 ? 4 : 3; }
+__host__ __device__ constexpr int prod_stages() { return 4; }
 template <int BM>
 constexpr size_t prod_smem(int split) {
     return 1024 + static_cast<size_t>(prod_stages<BM>()) * (TILE_N + BM) * KB + (split > 1 ? sizeof(int32_t) * TILE_N * BM : 0);
@@ -221,6 +277,157 @@ __global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant_
     }
 }
 
+// Many tokens: CTA pairs.  Two CTAs of a cluster share a tile of 256 channels x BM tokens through tcgen05 cta_group::2: each stages its
+// own 128 channels and half of the tokens, so the operands, whose way from L2 to the SMs binds 8-bit products, cross it once
+// per pair.  Persistent over tiles, two accumulators in tensor memory, so that one tile's epilogue runs under the next one's
+// MMAs.  Roles per CTA: TMA warp, MMA warp (the leader's issues for both), eight epilogue warps, two for each quarter of the
+// lanes.  Every TMA load counts on the leader's barrier; the leader's commits free the stages and hand the accumulators over in
+// both CTAs; epilogue warps of both release an accumulator on the leader's barrier.  All waits are bounded.
+constexpr int PAIR_THREADS = 64 + 32 * 8;
+constexpr int PAIR_CHANNELS = 256;
+template <int BM>
+__host__ __device__ constexpr int pair_stages() { return BM == 256 ? 6 : 8; }
+template <int BM>
+constexpr size_t pair_smem() { return 1024 + static_cast<size_t>(pair_stages<BM>()) * (TILE_N + BM / 2) * KB; }
+
+struct PairArgs {
+    ProductArgs p;
+    int32_t tiles_m, tiles, group;  // token tiles, all tiles, channel tiles that a wave of pairs walks together
+};
+// Tile number t: `group` channel tiles by all token tiles, channels innermost, so that the pairs at work at once share operands in L2.
+__device__ __forceinline__ void tile_place(const PairArgs& g, int32_t tiles_n, int32_t t, int32_t& tm, int32_t& tn) {
+    const int32_t per_band = g.group * g.tiles_m, band = t / per_band, width = min(g.group, tiles_n - band * g.group), in_band = t - band * per_band;
+    tm = in_band / width;
+    tn = band * g.group + in_band - tm * width;
+}
+
+template <int BM, class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    k_product_pair(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ PairArgs args) {
+    using namespace dense;
+    constexpr int STAGES = pair_stages<BM>();
+    constexpr uint32_t W_BYTES = TILE_N * KB, STAGE_BYTES = W_BYTES + BM / 2 * KB;
+    constexpr uint32_t TMEM_COLS = 2 * BM;
+    constexpr uint32_t IDESC = make_idesc(2, 1, PAIR_CHANNELS, BM);
+    const ProductArgs& g = args.p;
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base_slot;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int32_t first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1, tiles_n = args.tiles / args.tiles_m;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_base_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool alive = true;
+            for (int32_t tile = first_tile; tile < args.tiles && alive; tile += tile_step) {
+                int32_t tm, tn;
+                tile_place(args, tiles_n, tile, tm, tn);
+                const int32_t n0 = tn * PAIR_CHANNELS + static_cast<int32_t>(rank) * TILE_N, m0 = tm * BM + static_cast<int32_t>(rank) * (BM / 2);
+                for (int32_t kt = 0; kt < g.k_steps; ++kt) {
+                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, g.err, 1)) { alive = false; break; }
+                    if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+                    const uint32_t bar = peer_addr(smem_u32(&full_bar[stage]), 0);
+                    const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
+                    tma_load_2d_pair(dst, &map_w, bar, kt * KB, n0);
+                    tma_load_2d_pair(dst + W_BYTES, &map_a, bar, kt * KB, m0);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            uint32_t stage = 0, phase = 0, it = 0;
+            bool alive = true;
+            for (int32_t tile = first_tile; tile < args.tiles && alive; tile += tile_step, ++it) {
+                const uint32_t buf = it & 1u;
+                if (!mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, g.err, 2)) { alive = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t tmem_d = tmem + buf * BM;
+                for (int32_t kt = 0; kt < g.k_steps; ++kt) {
+                    if (!mbar_wait(&full_bar[stage], phase, g.err, 3)) { alive = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t w_addr = smem_u32(smem + stage * STAGE_BYTES);
+                    const uint64_t dw = make_smem_desc(w_addr), da = make_smem_desc(w_addr + W_BYTES);
+#pragma unroll
+                    for (int ks = 0; ks < KB / 32; ++ks)
+                        umma_pair<1>(tmem_d, dw + static_cast<uint64_t>(ks * 2), da + static_cast<uint64_t>(ks * 2), IDESC, (kt | ks) ? 1u : 0u);
+                    const uint32_t e = smem_u32(&empty_bar[stage]);
+                    umma_commit_pair(e);
+                    umma_commit_pair(peer_addr(e, 1));
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (alive) {
+                    const uint32_t f = smem_u32(&acc_full[buf]);
+                    umma_commit_pair(f);
+                    umma_commit_pair(peer_addr(f, 1));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2, ch = quarter * 32 + lane;
+        uint32_t it = 0;
+        for (int32_t tile = first_tile; tile < args.tiles; tile += tile_step, ++it) {
+            int32_t tm, tn;
+            tile_place(args, tiles_n, tile, tm, tn);
+            const uint32_t buf = it & 1u;
+            const int32_t col = tn * PAIR_CHANNELS + static_cast<int32_t>(rank) * TILE_N + ch, m0 = tm * BM + half * (BM / 2);
+            const float w_scale = col < g.n ? g.w_scale[col] : 0.0f, bias = g.bias && col < g.n ? g.bias[col] : 0.0f;
+            if (!mbar_wait(&acc_full[buf], (it >> 1) & 1u, g.err, 4)) break;
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t taddr = tmem + buf * BM + half * (BM / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
+            T* out = static_cast<T*>(g.out) + static_cast<int64_t>(m0) * g.out_pitch + col;
+#pragma unroll 1
+            for (int c = 0; c < BM / 32; ++c) {
+                uint32_t acc[16];
+                tmem_ld16_issue(taddr + c * 16, acc);
+                tmem_ld_wait();
+                const int32_t left = g.m - (m0 + c * 16);  // tokens from here on
+                if (col < g.n)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (j < left) {
+                            const float y = __int2float_rn(static_cast<int32_t>(acc[j])) * __ldg(g.a_scale + m0 + c * 16 + j) * w_scale;
+                            out[(c * 16 + j) * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
+                        }
+                __syncwarp();
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(peer_addr(smem_u32(&acc_empty[buf]), 0));
+        }
+        __syncwarp();
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();  // no CTA leaves (or frees tensor memory) while its peer can still reach it
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
 struct Product {
     int64_t m, n, k;
     const int8_t* a;
@@ -275,16 +482,35 @@ int32_t launch_product(thrml_ctx* ctx, cudaStream_t stream, const Product& p, in
     return THRML_OK;
 }
 
+template <int BM, class T>
+int32_t launch_pair(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
+    CUtensorMap map_w, map_a;
+    if (int32_t rc = make_operand_map(&map_w, const_cast<int8_t*>(p.w), true, p.k, p.n, p.w_pitch, TILE_N)) return rc;
+    if (int32_t rc = make_operand_map(&map_a, const_cast<int8_t*>(p.a), true, p.k, p.m, p.a_pitch, BM / 2)) return rc;
+    const int32_t tiles_m = static_cast<int32_t>((p.m + BM - 1) / BM), tiles_n = static_cast<int32_t>((p.n + PAIR_CHANNELS - 1) / PAIR_CHANNELS);
+    const PairArgs g{{static_cast<int32_t>(p.m), static_cast<int32_t>(p.n), static_cast<int32_t>((p.k + KB - 1) / KB), p.a_scale, p.w_scale, p.bias, p.out, p.out_pitch, ctx->wait_flag_dev},
+                     tiles_m, tiles_m * tiles_n, 8};
+    CU_TRY(cudaFuncSetAttribute(k_product_pair<BM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pair_smem<BM>())));
+    const int pairs = std::min(ctx->sm_count / 2, tiles_m * tiles_n);
+    k_product_pair<BM, T><<<2 * pairs, PAIR_THREADS, pair_smem<BM>(), stream>>>(map_w, map_a, g);
+    CU_TRY(cudaGetLastError());
+    return THRML_OK;
+}
+
 template <class T>
 int32_t product(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
-    const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+    // Pairs from 65 tokens on: 256 tokens a tile where that leaves a tile for each of them, else 128.
+    if (p.m > 64) {
+        const int64_t wide = (p.n + PAIR_CHANNELS - 1) / PAIR_CHANNELS * ((p.m + 255) / 256);
+        return wide >= ctx->sm_count / 2 ? launch_pair<256, T>(ctx, stream, p) : launch_pair<128, T>(ctx, stream, p);
+    }
+    const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : 64;
     const int64_t tiles = (p.n + TILE_N - 1) / TILE_N * ((p.m + bm - 1) / bm), k_steps = (p.k + KB - 1) / KB;
     int split = 1;
     while (split < 8 && tiles * split < 2 * ctx->sm_count && 2 * split <= k_steps) split *= 2;
     if (bm == 16) return launch_product<16, T>(ctx, stream, p, split);
     if (bm == 32) return launch_product<32, T>(ctx, stream, p, split);
-    if (bm == 64) return launch_product<64, T>(ctx, stream, p, split);
-    return launch_product<128, T>(ctx, stream, p, split);
+    return launch_product<64, T>(ctx, stream, p, split);
 }
 
 int32_t run_product(thrml_ctx* ctx, void* stream, const Product& p) {
@@ -315,7 +541,9 @@ int32_t run_quant(void* stream, const Quant& z) {
     if (z.rows == 0) return THRML_OK;
     const QuantArgs g{z.x, z.x_pitch, z.q, z.q_pitch, z.scale, static_cast<int32_t>(z.cols)};
     return for_type(z.x_type, [&](auto e) {
-        k_quantize<decltype(e)><<<static_cast<unsigned>(z.rows), QUANT_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(g);
+        int threads = 32;
+        while (threads < QUANT_THREADS && static_cast<int64_t>(threads) * QUANT_PIECES * VEC<decltype(e)> < z.cols) threads *= 2;
+        k_quantize<decltype(e)><<<static_cast<unsigned>(z.rows), threads, 0, static_cast<cudaStream_t>(stream)>>>(g);
         CU_TRY(cudaGetLastError());
         return THRML_OK;
     });
