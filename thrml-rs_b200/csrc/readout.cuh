@@ -205,6 +205,16 @@ int32_t guarded(thrml_ctx* ctx, F body) noexcept {
     }
 }
 
+// Lets a kernel have more than 48 KB of dynamic shared memory, once for each device.
+template <auto KERNEL>
+int32_t allow_shared(const thrml_ctx* ctx, size_t bytes) {
+    static bool done[64] = {};
+    if (ctx->device < 64 && done[ctx->device]) return THRML_OK;
+    CU_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    if (ctx->device < 64) done[ctx->device] = true;
+    return THRML_OK;
+}
+
 // f(element of the type) for one of the three float types.
 template <class F>
 int32_t for_type(int32_t type, F f) {

@@ -967,7 +967,7 @@ int32_t thrml_adjust_logits(thrml_ctx* ctx, void* stream, int64_t rows, int64_t 
             const int64_t count_bytes = std::max<int64_t>(2 * share, 4 * std::min<int64_t>(share, ADJUST_SHARE<T> / 2));
             const AdjustArgs g{logits, out, pitch, out_pitch, static_cast<int32_t>(cols), static_cast<int32_t>(share), static_cast<int32_t>(per_row), static_cast<int32_t>(count_bytes / 4), *rules};
             const size_t smem = 16 * ADJUST_PIECES * ADJUST_THREADS + (rules->history ? count_bytes : 0) + (rules->bias_ids ? share / 8 : 0);
-            CU_TRY(cudaFuncSetAttribute(k_adjust<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * ADJUST_PIECES * ADJUST_THREADS + ADJUST_SHARE<T> * 2 + ADJUST_SHARE<T> / 8));
+            if (int32_t rc = allow_shared<k_adjust<T>>(ctx, 16 * ADJUST_PIECES * ADJUST_THREADS + ADJUST_SHARE<T> * 2 + ADJUST_SHARE<T> / 8)) return rc;
             k_adjust<T><<<static_cast<unsigned>(rows * per_row), ADJUST_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(g);
             CU_TRY(cudaGetLastError());
             return THRML_OK;

@@ -185,8 +185,16 @@ __global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant_
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            for (int32_t kt = k_begin; kt < k_end; ++kt) {
+            // The weights of the first stages do not wait for the kernel that quantises the tokens.
+            const int32_t early = min(k_end - k_begin, STAGES);
+            for (int32_t i = 0; i < early; ++i) {
+                mbar_expect_tx(&full_bar[i], STAGE_BYTES);
+                tma_load_2d(smem_u32(smem + i * STAGE_BYTES), &map_w, &full_bar[i], (k_begin + i) * KB, n0);
+            }
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int32_t i = 0; i < early; ++i) tma_load_2d(smem_u32(smem + i * STAGE_BYTES) + W_BYTES, &map_a, &full_bar[i], (k_begin + i) * KB, m0);
+            uint32_t stage = early == STAGES ? 0 : early, phase = early == STAGES ? 1 : 0;
+            for (int32_t kt = k_begin + early; kt < k_end; ++kt) {
                 if (!mbar_wait(&empty_bar[stage], phase ^ 1u, g.err, 1)) break;
                 mbar_expect_tx(&full_bar[stage], STAGE_BYTES);
                 const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
@@ -225,6 +233,7 @@ __global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant_
                 out[token * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
             }
         };
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' scales
         const bool alive = mbar_wait(&acc_full, 0, g.err, 4);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -343,7 +352,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 int32_t tm, tn;
                 tile_place(args, tiles_n, tile, tm, tn);
                 const int32_t n0 = tn * PAIR_CHANNELS + static_cast<int32_t>(rank) * TILE_N, m0 = tm * BM + static_cast<int32_t>(rank) * (BM / 2);
-                for (int32_t kt = 0; kt < g.k_steps; ++kt) {
+                int32_t early = 0;
+                if (tile == first_tile) {  // the weights of the first stages do not wait for the kernel that quantises the tokens
+                    early = min(g.k_steps, STAGES);
+                    for (int32_t i = 0; i < early; ++i) {
+                        if (leader) mbar_expect_tx(&full_bar[i], 2 * STAGE_BYTES);
+                        tma_load_2d_pair(smem_u32(smem + i * STAGE_BYTES), &map_w, peer_addr(smem_u32(&full_bar[i]), 0), i * KB, n0);
+                    }
+                    asm volatile("griddepcontrol.wait;" ::: "memory");
+                    for (int32_t i = 0; i < early; ++i)
+                        tma_load_2d_pair(smem_u32(smem + i * STAGE_BYTES) + W_BYTES, &map_a, peer_addr(smem_u32(&full_bar[i]), 0), i * KB, m0);
+                    stage = early == STAGES ? 0 : early;
+                    phase = early == STAGES ? 1 : 0;
+                }
+                for (int32_t kt = early; kt < g.k_steps; ++kt) {
                     if (!mbar_wait(&empty_bar[stage], phase ^ 1u, g.err, 1)) { alive = false; break; }
                     if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
                     const uint32_t bar = peer_addr(smem_u32(&full_bar[stage]), 0);
@@ -388,6 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2, ch = quarter * 32 + lane;
         uint32_t it = 0;
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' scales
         for (int32_t tile = first_tile; tile < args.tiles; tile += tile_step, ++it) {
             int32_t tm, tn;
             tile_place(args, tiles_n, tile, tm, tn);
@@ -440,6 +463,7 @@ struct Product {
     void* out;
     int32_t out_type;
     int64_t out_pitch;
+    bool after_quantising;  // the launch before is k_quantize, which lets this one start early
 };
 
 int32_t check_matrix8(const char* what, const void* p, int64_t k, int64_t pitch) {
@@ -467,17 +491,19 @@ int32_t launch_product(thrml_ctx* ctx, cudaStream_t stream, const Product& p, in
     if (int32_t rc = make_operand_map(&map_w, const_cast<int8_t*>(p.w), true, p.k, p.n, p.w_pitch, TILE_N)) return rc;
     if (int32_t rc = make_operand_map(&map_a, const_cast<int8_t*>(p.a), true, p.k, p.m, p.a_pitch, BM)) return rc;
     ProductArgs g{static_cast<int32_t>(p.m), static_cast<int32_t>(p.n), static_cast<int32_t>((p.k + KB - 1) / KB), p.a_scale, p.w_scale, p.bias, p.out, p.out_pitch, ctx->wait_flag_dev};
-    CU_TRY(cudaFuncSetAttribute(k_product<BM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(prod_smem<BM>(2))));
+    if (int32_t rc = allow_shared<k_product<BM, T>>(ctx, static_cast<int>(prod_smem<BM>(2)))) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((p.n + TILE_N - 1) / TILE_N * split), static_cast<unsigned>((p.m + BM - 1) / BM));
     cfg.blockDim = dim3(PROD_THREADS);
     cfg.dynamicSmemBytes = prod_smem<BM>(split);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {static_cast<unsigned>(split), 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = p.after_quantising ? 2 : 1;
     CU_TRY(cudaLaunchKernelEx(&cfg, k_product<BM, T>, map_w, map_a, g));
     return THRML_OK;
 }
@@ -490,10 +516,19 @@ int32_t launch_pair(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
     const int32_t tiles_m = static_cast<int32_t>((p.m + BM - 1) / BM), tiles_n = static_cast<int32_t>((p.n + PAIR_CHANNELS - 1) / PAIR_CHANNELS);
     const PairArgs g{{static_cast<int32_t>(p.m), static_cast<int32_t>(p.n), static_cast<int32_t>((p.k + KB - 1) / KB), p.a_scale, p.w_scale, p.bias, p.out, p.out_pitch, ctx->wait_flag_dev},
                      tiles_m, tiles_m * tiles_n, 8};
-    CU_TRY(cudaFuncSetAttribute(k_product_pair<BM, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pair_smem<BM>())));
+    if (int32_t rc = allow_shared<k_product_pair<BM, T>>(ctx, static_cast<int>(pair_smem<BM>()))) return rc;
     const int pairs = std::min(ctx->sm_count / 2, tiles_m * tiles_n);
-    k_product_pair<BM, T><<<2 * pairs, PAIR_THREADS, pair_smem<BM>(), stream>>>(map_w, map_a, g);
-    CU_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+    cfg.blockDim = dim3(PAIR_THREADS);
+    cfg.dynamicSmemBytes = pair_smem<BM>();
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = p.after_quantising ? 1 : 0;
+    CU_TRY(cudaLaunchKernelEx(&cfg, k_product_pair<BM, T>, map_w, map_a, g));
     return THRML_OK;
 }
 
@@ -565,7 +600,7 @@ int32_t thrml_quantize_rows_i8(thrml_ctx* ctx, void* stream, int64_t rows, int64
 int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* w,
                         int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch) {
     return guarded(ctx, [&]() -> int32_t {
-        const Product p{m, n, k, a, a_pitch, a_scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch};
+        const Product p{m, n, k, a, a_pitch, a_scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch, false};
         if (int32_t rc = check_product(p)) return rc;
         return run_product(ctx, stream, p);
     });
@@ -574,7 +609,7 @@ int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int6
 int32_t thrml_linear_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
                         float* scale, const int8_t* w, int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch) {
     return guarded(ctx, [&]() -> int32_t {
-        const Product p{m, n, k, q, q_pitch, scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch};
+        const Product p{m, n, k, q, q_pitch, scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch, true};
         if (int32_t rc = check_product(p)) return rc;
         const Quant z{m, k, x, x_type, x_pitch, q, q_pitch, scale};
         if (int32_t rc = check_quant(z)) return rc;
