@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(QUANT_THREADS) k_quantize(const __grid_constan
 // ---------------------------------------------------------------------------------------------------------
 constexpr int TILE_N = 128;  // channels of a tile = tensor-memory lanes
 constexpr int KB = 128;      // bytes of K per stage: one 128-byte swizzle atom
-constexpr int PROD_THREADS = 192;  // TMA warp, MMA warp, four epilogue warps
+template <int BM>
+constexpr int PROD_THREADS = BM == 16 ? 192 : 320;  // TMA warp, MMA warp, four epilogue warps (eight where there are two or more pieces of 16 tokens)
 
 struct ProductArgs {
     int32_t m, n, k_steps;
@@ -139,7 +140,7 @@ struct ProductArgs {
 };
 
 template <int BM>
-__host__ __device__ constexpr int prod_stages() { return 4; }
+__host__ __device__ constexpr int prod_stages() { return BM == 64 ? 4 : 5; }  // two CTAs an SM: with three or four, calls one behind the other took up to three times as long
 template <int BM>
 constexpr size_t prod_smem(int split) {
     return 1024 + static_cast<size_t>(prod_stages<BM>()) * (TILE_N + BM) * KB + (split > 1 ? sizeof(int32_t) * TILE_N * BM : 0);
@@ -149,7 +150,7 @@ constexpr size_t prod_smem(int split) {
 // a row of the output, and few tokens still fill the MMA's 128 rows.  The CTAs of a cluster (1, 2, 4 or 8) share a tile:
 // each takes a part of K, hands its 32-bit sums over through distributed shared memory, and finishes a part of the tokens.
 template <int BM, class T>
-__global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const ProductArgs g) {
+__global__ void __launch_bounds__(PROD_THREADS<BM>) k_product(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const ProductArgs g) {
     using namespace dense;
     constexpr int STAGES = prod_stages<BM>();
     constexpr uint32_t W_BYTES = TILE_N * KB, STAGE_BYTES = W_BYTES + BM * KB;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant_
         int32_t* red = reinterpret_cast<int32_t*>(smem + STAGES * STAGE_BYTES);  // [source CTA][token of the share][channel]
         const int32_t share = BM / static_cast<int32_t>(split);
         __syncwarp();
-        for (int c = 0; c < BM / 16; ++c) {
+        for (int c = (warp - 2) >> 2; c < BM / 16; c += (PROD_THREADS<BM> - 64) / 128) {
             uint32_t acc[16];
             tmem_ld16_issue(taddr + c * 16, acc);
             tmem_ld_wait();
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant_
             if (col < g.n) {
                 const float w_scale = g.w_scale[col], bias = g.bias ? g.bias[col] : 0.0f;
                 T* out = static_cast<T*>(g.out) + col;
-                for (int32_t t = 0; t < share; ++t) {
+                for (int32_t t = (warp - 2) >> 2; t < share; t += (PROD_THREADS<BM> - 64) / 128) {
                     const int32_t token = m0 + static_cast<int32_t>(rank) * share + t;
                     if (token >= g.m) break;
                     int32_t acc = 0;
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(PROD_THREADS) k_product(const __grid_constant_
 constexpr int PAIR_THREADS = 64 + 32 * 8;
 constexpr int PAIR_CHANNELS = 256;
 template <int BM>
-__host__ __device__ constexpr int pair_stages() { return BM == 256 ? 6 : 8; }
+__host__ __device__ constexpr int pair_stages() { return 192 * 1024 / ((TILE_N + BM / 2) * KB); }
 template <int BM>
 constexpr size_t pair_smem() { return 1024 + static_cast<size_t>(pair_stages<BM>()) * (TILE_N + BM / 2) * KB; }
 
@@ -494,7 +495,7 @@ int32_t launch_product(thrml_ctx* ctx, cudaStream_t stream, const Product& p, in
     if (int32_t rc = allow_shared<k_product<BM, T>>(ctx, static_cast<int>(prod_smem<BM>(2)))) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((p.n + TILE_N - 1) / TILE_N * split), static_cast<unsigned>((p.m + BM - 1) / BM));
-    cfg.blockDim = dim3(PROD_THREADS);
+    cfg.blockDim = dim3(PROD_THREADS<BM>);
     cfg.dynamicSmemBytes = prod_smem<BM>(split);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -534,15 +535,18 @@ int32_t launch_pair(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
 
 template <class T>
 int32_t product(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
-    // Pairs from 65 tokens on: 256 tokens a tile where that leaves a tile for each of them, else 128.
+    // Pairs from 65 tokens on: 256 tokens a tile where that leaves a tile for each of them, else 128.  Up to 64 tokens the
+    // weights' way from memory is what binds, and two CTAs an SM keep more of them in flight (4096 inputs, 65536 channels: 16
+    // tokens 47 us, in pairs 58; 64 tokens 53, in pairs 61).
     if (p.m > 64) {
         const int64_t wide = (p.n + PAIR_CHANNELS - 1) / PAIR_CHANNELS * ((p.m + 255) / 256);
         return wide >= ctx->sm_count / 2 ? launch_pair<256, T>(ctx, stream, p) : launch_pair<128, T>(ctx, stream, p);
     }
+    // K is split while that takes no more than the SMs.
     const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : 64;
-    const int64_t tiles = (p.n + TILE_N - 1) / TILE_N * ((p.m + bm - 1) / bm), k_steps = (p.k + KB - 1) / KB;
+    const int64_t tiles = (p.n + TILE_N - 1) / TILE_N, k_steps = (p.k + KB - 1) / KB;
     int split = 1;
-    while (split < 8 && tiles * split < 2 * ctx->sm_count && 2 * split <= k_steps) split *= 2;
+    while (split < 8 && 2 * tiles * split <= ctx->sm_count && 2 * split <= k_steps) split *= 2;
     if (bm == 16) return launch_product<16, T>(ctx, stream, p, split);
     if (bm == 32) return launch_product<32, T>(ctx, stream, p, split);
     return launch_product<64, T>(ctx, stream, p, split);
