@@ -110,7 +110,7 @@ def product64(q, qs, w, ws, b, dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 16, 17), (2, 128, 127), (1, 4096, 129), (16, 784, 300), (17, 31, 128), (31, 513, 1000), (33, 784, 4097), (64, 1024, 640), (65, 256, 257), (127, 2049, 130), (128, 128, 128),
-          (129, 300, 385), (257, 130, 1025), (511, 1000, 77), (513, 4096, 513), (1000, 96, 2000), (2049, 333, 515)]
+          (129, 300, 385), (257, 130, 1025), (511, 1000, 77), (513, 4096, 513), (1000, 96, 2000), (2049, 333, 515), (5000, 200, 700), (6300, 130, 761), (3000, 1030, 1500)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)

@@ -535,16 +535,17 @@ int32_t launch_pair(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
 
 template <class T>
 int32_t product(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
-    // Pairs from 65 tokens on: 256 tokens a tile where that leaves a tile for each of them, else 128.  Up to 64 tokens the
-    // weights' way from memory is what binds, and two CTAs an SM keep more of them in flight (4096 inputs, 65536 channels: 16
-    // tokens 47 us, in pairs 58; 64 tokens 53, in pairs 61).
-    if (p.m > 64) {
-        const int64_t wide = (p.n + PAIR_CHANNELS - 1) / PAIR_CHANNELS * ((p.m + 255) / 256);
-        return wide >= ctx->sm_count / 2 ? launch_pair<256, T>(ctx, stream, p) : launch_pair<128, T>(ctx, stream, p);
+    // Up to 64 tokens, and up to a wave of two CTAs an SM, the operands' way from memory binds, and many CTAs keep more of them
+    // in flight (4096 inputs, 65536 channels: 16 tokens 47 us, in pairs 58; 64 tokens 53, in pairs 61; 4096 channels: 128 tokens
+    // 15, in pairs 20; 512 tokens 19, in pairs 22).  Beyond, pairs: with 256 tokens a tile unless 128 need fewer rounds for the
+    // half of the work each.
+    const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : 64;
+    const int64_t tiles = (p.n + TILE_N - 1) / TILE_N * ((p.m + bm - 1) / bm), k_steps = (p.k + KB - 1) / KB;
+    if (p.m > 64 && tiles > 2 * ctx->sm_count) {
+        const auto rounds = [&](int64_t width) { return ((p.n + PAIR_CHANNELS - 1) / PAIR_CHANNELS * ((p.m + width - 1) / width) + ctx->sm_count / 2 - 1) / (ctx->sm_count / 2); };
+        return 2 * rounds(256) <= rounds(128) ? launch_pair<256, T>(ctx, stream, p) : launch_pair<128, T>(ctx, stream, p);
     }
     // K is split while that takes no more than the SMs.
-    const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : 64;
-    const int64_t tiles = (p.n + TILE_N - 1) / TILE_N, k_steps = (p.k + KB - 1) / KB;
     int split = 1;
     while (split < 8 && 2 * tiles * split <= ctx->sm_count && 2 * split <= k_steps) split *= 2;
     if (bm == 16) return launch_product<16, T>(ctx, stream, p, split);
