@@ -608,6 +608,66 @@ def test_on_another_stream_and_in_two_graphs(T):
     assert all(torch.equal(a, b) for a, b in zip(outs[0], fresh))
 
 
+def test_offsets_past_32_bits(T):
+    """Rows 2^30 + 16 elements apart: the third begins past 2^31."""
+    v, pitch = 5000, (1 << 30) + 16
+    space = torch.empty(2 * pitch + v, dtype=torch.bfloat16, device="cuda")
+    far = space.as_strided((3, v), (pitch, 1))
+    x = torch.randn(3, v, generator=gen(1), device="cuda").bfloat16()
+    far.copy_(x)
+    rules, beta = make_rules(3, v, 1), torch.ones(3, device="cuda")
+    _, ids, teacher, _ = make_distill(3, v, 7, 1, torch.bfloat16)
+    assert torch.equal(T.draw_categories(far, 3, beta=beta), T.draw_categories(x, 3, beta=beta))
+    q, s = T.quantize_rows(x)
+    assert all(torch.equal(a, b) for a, b in zip(T.quantize_rows(far), (q, s)))
+    loss, grad = T.distill_step(x, ids, teacher)
+    loss2, grad2 = T.distill_step(far, ids, teacher)
+    assert torch.equal(loss, loss2) and torch.equal(grad, grad2)
+    want = T.adjust_logits(x, **rules)
+    T.adjust_logits(far, **rules, out=far)
+    assert torch.equal(far, want)
+    lse = T.distill_loss(x, ids, teacher)[1]
+    T.distill_grad(x, lse, ids, teacher, out=far)
+    near(far, grad, 4 * half(torch.bfloat16) * grad.abs().double() + 1e-6)
+    w, ws = T.quantize_rows(torch.randn(v, v, generator=gen(2), device="cuda"))
+    T.int8_matmul(q, s, w, ws, out=far)
+    assert torch.equal(far, T.int8_matmul(q, s, w, ws, out_dtype=torch.bfloat16))
+    many = torch.randn(700, v, generator=gen(3), device="cuda").bfloat16()  # the kernel of many tokens, a column per 2^22 elements
+    wide = torch.empty(700 * (1 << 22), dtype=torch.bfloat16, device="cuda").as_strided((700, v), (1 << 22, 1))
+    T.int8_linear(many, w, ws, out=wide)
+    assert torch.equal(wide, T.int8_linear(many, w, ws))
+
+
+def test_ids_past_32_bits_are_padding(T):
+    x = torch.randn(2, 300, generator=gen(1), device="cuda")
+    h = torch.tensor([5, (1 << 40) + 5, -(1 << 40) + 7, 1 << 32, 8, 5], device="cuda")
+    rules = dict(history=h, history_ptr=torch.tensor([0, 6, 6], device="cuda"), frequency=torch.ones(2, device="cuda"))
+    clean = dict(rules, history=torch.tensor([5, 8, 5], device="cuda"), history_ptr=torch.tensor([0, 3, 3], device="cuda"))
+    assert torch.equal(T.adjust_logits(x, **rules), T.adjust_logits(x, **clean))
+    ids = torch.tensor([[3, (1 << 40) + 3, -1]], device="cuda").repeat(2, 1)
+    teacher = torch.zeros(2, 3, device="cuda")
+    a, b = T.distill_step(x, ids, teacher), T.distill_step(x, ids[:, :1], teacher[:, :1])
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+
+
+def test_current_device_and_errors_stay_the_callers(T):
+    """A refused call leaves no error behind, and the current device does not change."""
+    before = torch.cuda.current_device()
+    x = torch.randn(4, 100, device="cuda")
+    with pytest.raises(T.ThrmlError):
+        T.draw_categories(x, 1, row_offset=1 << 33)
+    T.draw_categories(x, 1)
+    assert torch.cuda.current_device() == before and bool((x + 1).isfinite().all())
+
+
+def test_context_reports_no_wait_that_ran_out(T):
+    from thrml_rs_b200 import engine
+    q, s = T.quantize_rows(torch.randn(70, 300, device="cuda"))
+    T.int8_matmul(q, s, q, s)
+    torch.cuda.synchronize()
+    engine.default_context(0).synchronize()  # would raise THRML_ERR_TIMEOUT
+
+
 def test_refused_on_the_gpu(T):
     x = torch.zeros(4, 64, device="cuda")
     w = torch.zeros(8, 64, dtype=torch.int8, device="cuda")

@@ -197,7 +197,9 @@ int32_t guarded(thrml_ctx* ctx, F body) noexcept {
         if (int32_t rc = ctx->check_waits()) return rc;
         OnDevice on(ctx->device);
         CU_TRY(on.status());
-        return body();
+        const int32_t rc = body();
+        if (rc == THRML_ERR_CUDA) cudaGetLastError();  // a refused launch is reported here, not by whoever asks next
+        return rc;
     } catch (const std::bad_alloc&) {
         return THRML_ERR_OOM;  // no message: making one would allocate
     } catch (...) {

@@ -970,8 +970,12 @@ int32_t thrml_adjust_logits(thrml_ctx* ctx, void* stream, int64_t rows, int64_t 
             const AdjustArgs g{logits, out, pitch, out_pitch, static_cast<int32_t>(cols), static_cast<int32_t>(share), static_cast<int32_t>(per_row), static_cast<int32_t>(count_bytes / 4), *rules};
             const size_t smem = 16 * ADJUST_PIECES * ADJUST_THREADS + (rules->history ? count_bytes : 0) + (rules->bias_ids ? share / 8 : 0);
             if (int32_t rc = allow_shared<k_adjust<T>>(ctx, 16 * ADJUST_PIECES * ADJUST_THREADS + ADJUST_SHARE<T> * 2 + ADJUST_SHARE<T> / 8)) return rc;
-            k_adjust<T><<<static_cast<unsigned>(rows * per_row), ADJUST_THREADS, smem, static_cast<cudaStream_t>(stream)>>>(g);
-            CU_TRY(cudaGetLastError());
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(static_cast<unsigned>(rows * per_row));
+            cfg.blockDim = dim3(ADJUST_THREADS);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream = static_cast<cudaStream_t>(stream);
+            CU_TRY(cudaLaunchKernelEx(&cfg, k_adjust<T>, g));
             return THRML_OK;
         });
     });

@@ -583,8 +583,11 @@ int32_t run_quant(void* stream, const Quant& z) {
     return for_type(z.x_type, [&](auto e) {
         int threads = 32;
         while (threads < QUANT_THREADS && static_cast<int64_t>(threads) * QUANT_PIECES * VEC<decltype(e)> < z.cols) threads *= 2;
-        k_quantize<decltype(e)><<<static_cast<unsigned>(z.rows), threads, 0, static_cast<cudaStream_t>(stream)>>>(g);
-        CU_TRY(cudaGetLastError());
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(z.rows));
+        cfg.blockDim = dim3(static_cast<unsigned>(threads));
+        cfg.stream = static_cast<cudaStream_t>(stream);
+        CU_TRY(cudaLaunchKernelEx(&cfg, k_quantize<decltype(e)>, g));
         return THRML_OK;
     });
 }
