@@ -125,6 +125,7 @@ template <class T>
 __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_constant__ AdjustArgs g) {
     constexpr int V = VEC<T>;
     extern __shared__ uint4 adjust_smem[];
+    __shared__ uint32_t mask_words[ADJUST_SHARE<T> / 32 + 2];
     const int tid = threadIdx.x;
     const thrml_logit_rules& ru = g.rules;
     const int64_t row = g.per_row == 1 ? blockIdx.x : blockIdx.x / g.per_row;
@@ -155,6 +156,11 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
     const uint32_t* mask = ru.mask && m >= 0 && m < ru.n_masks ? ru.mask + m * ru.mask_pitch : nullptr;
     const bool wide = pieces.same_phase(out);
     float logit = 0.0f;  // of the first bias entry that this thread finishes, read early
+    if (has_history)
+        for (int i = tid; i < g.count_words / 4; i += ADJUST_THREADS) counts[i] = make_uint4(0u, 0u, 0u, 0u);
+    const int32_t first_word = max(from - ahead, 0) >> 5;  // of the mask, which the share needs up to the word of its last category
+    if (mask)
+        for (int32_t i = first_word + tid; i <= (to - 1 - ahead) >> 5; i += ADJUST_THREADS) mask_words[i - first_word] = mask[i];
     if (has_bias) {
         for (int i = tid; i < g.share / 32; i += ADJUST_THREADS) biased[i] = 0u;
         __syncthreads();
@@ -171,8 +177,9 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
         constexpr int BITS = decltype(bits)::value;
         const Counts<BITS> count{reinterpret_cast<uint32_t*>(counts)};
         if (has_history) {
-            for (int i = tid; i < (stop - begin + 128 / BITS - 1) / (128 / BITS); i += ADJUST_THREADS) counts[i] = make_uint4(0u, 0u, 0u, 0u);
-            __syncthreads();
+            if (s0 > 0)  // the second half's; the first begin at 0
+                for (int i = tid; i < g.count_words / 4; i += ADJUST_THREADS) counts[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (s0 > 0 || !has_bias) __syncthreads();
             // `low` is the category at `begin`; below 0 (the first CTA's, when ahead > 0) lie no categories
             const int32_t low = max(begin - ahead, 0);
             const uint32_t first = low + ahead - begin, n = static_cast<uint32_t>(stop - ahead - low);
@@ -233,8 +240,9 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
             uint4 bits = raw;
             if (mask) {
                 const int32_t k0 = max(k, 0);  // the first piece of a row may begin before it
-                uint32_t open = mask[k0 >> 5] >> (k0 & 31);
-                if ((k0 & 31) + V > 32 && ((k0 >> 5) + 1) * 32 < g.cols) open |= mask[(k0 >> 5) + 1] << (32 - (k0 & 31));
+                const uint32_t* w = mask_words + (k0 >> 5) - first_word;
+                uint32_t open = w[0] >> (k0 & 31);
+                if ((k0 & 31) + V > 32) open |= w[1] << (32 - (k0 & 31));  // behind the row's last word: bits that are not used
                 bits = close_16<T>(bits, open << (k0 - k));
             }
             const uint32_t done = has_bias ? biased[(at - from) >> 5] >> ((at - from) & 31) & ((1u << V) - 1u) : 0u;  // V positions lie in one word
