@@ -536,7 +536,8 @@ int32_t thrml_quantize_rows_i8(thrml_ctx* ctx, void* stream, int64_t rows, int64
  * once to out_type.  a and w start on 16-byte boundaries and their pitches are multiples of 16. */
 int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* w,
                         int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch);
-/* Both: x is quantised into q (16-byte boundary, pitch a multiple of 16) and scale, the caller's workspaces, then multiplied. */
+/* Both: x is quantised, then multiplied.  q (16-byte boundary, pitch a multiple of 16) and scale are the caller's workspaces; what
+ * they hold afterwards is not specified. */
 int32_t thrml_linear_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
                         float* scale, const int8_t* w, int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch);
 /* The rules of one generation step on logits[rows][cols], in this order (all in f32, rounded once to the logits' type):

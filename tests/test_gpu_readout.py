@@ -161,6 +161,25 @@ def test_int8_linear(T, dtype, m, k, n):
     near(T.int8_linear(x, wq, wsc, out_dtype=torch.float32), (q * s[:, None]) @ q64.T, 8 * E * (q * s[:, None]).abs() @ q64.abs().T + 1e-30)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m, k, n", [(1, 8, 1), (1, 4096, 513), (2, 4096, 4096), (16, 512, 300), (3, 24, 40), (1, 8192, 130), (8, 1000, 77), (5, 136, 20000), (7, 128, 129)])
+def test_int8_linear_of_few_tokens(T, dtype, m, k, n):
+    """Small products quantise their tokens themselves: what the two calls give, rows of zeros and of infinities among them."""
+    g = gen(m * k + n)
+    x = (torch.randn(m, k, generator=g, device="cuda") * torch.logspace(-3, 3, m, device="cuda")[:, None]).to(dtype)
+    if m > 2:
+        x[1] = 0
+        x[2, k // 2] = math.inf
+    w, ws = T.quantize_rows(torch.randn(n, k, generator=g, device="cuda"))
+    b = torch.randn(n, generator=g, device="cuda")
+    q, s = T.quantize_rows(x)
+    for out_dtype in TYPES:
+        got, want = T.int8_linear(x, w, ws, b, out_dtype=out_dtype), T.int8_matmul(q, s, w, ws, b, out_dtype=out_dtype)
+        assert torch.equal(got.nan_to_num(12345.0), want.nan_to_num(12345.0)) and bool((got.isnan() == want.isnan()).all())
+    if m > 2:
+        assert got[2].isnan().all() and torch.equal(got[1], b.to(out_dtype))
+
+
 # ---- rules
 
 
