@@ -56,7 +56,7 @@ __device__ __forceinline__ void unpack_16(const uint4& raw, float (&v)[VEC<T>]) 
             v[2 * i] = f.x, v[2 * i + 1] = f.y;
         } else {
             // a bf16 is the upper half of its f32: shift and mask, where the conversion instruction would run on the pipe that
-            // the exponentials need (a 256 x 131072 draw took 65 us with it)
+            // the exponentials need
             v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
