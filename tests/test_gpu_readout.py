@@ -46,6 +46,8 @@ def near(got, want, tol):
     got, want = got.double(), want.double()
     assert got.shape == want.shape
     same = (got == want) | (got.isnan() & want.isnan())
+    # Every number within the tolerance is as good as the value; from (2 - 2^-24) 2^127 on, f32 rounds them to infinity.
+    same |= got.isinf() & (got.sign() == want.sign()) & (want.abs() + tol >= (2 - 2.0**-24) * 2.0**127)
     ok = same | ((got - want).abs() <= tol)
     assert bool(ok.all()), f"{int((~ok).sum())} values, worst {((got - want).abs() / tol)[~ok].max()} tolerances off"
 
@@ -527,6 +529,44 @@ def test_distill_rows_of_the_lowest_value(T, dtype, v):
             rows = (0, 1, 2) if dtype != torch.float16 else (1, )  # f16's ends are ordinary numbers: lse holds the row's size to 2^-8 only
             for i in rows:
                 near(grad[i], want[i], half(dtype) * want[i].abs() + E * 64 * beta + TINY[dtype])
+
+
+@pytest.mark.parametrize("rows", [3, 700])  # few rows: one launch; many: the lists in their own
+@pytest.mark.parametrize("top", [1, 33, 64, 65, 129, 1024])
+@pytest.mark.parametrize("several", [1, 3, 40, 1000])
+def test_distill_categories_listed_again(T, rows, top, several):
+    """Lists that take up few categories again and again, in every order, with entries that are not listed among them."""
+    v = 2003
+    x, _, teacher, weight = make_distill(rows, v, top, rows + top, torch.bfloat16)
+    g = gen(several)
+    of = torch.randint(0, v, (rows, several), generator=g, device="cuda")
+    ids = of.gather(1, torch.randint(0, several, (rows, top), generator=g, device="cuda"))
+    ids[torch.rand(rows, top, generator=g, device="cuda") < 0.1] = -1
+    loss, lse, grad = check_distill(T, x, ids, teacher, 0.8, weight)
+    again = T.distill_loss(x, ids, teacher, beta=0.8, weight=weight)[0], T.distill_grad(x, lse, ids, teacher, beta=0.8, weight=weight)
+    assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [6, 70])
+def test_distill_odd_rows_among_many(T, dtype, top):
+    """The odd rows again, where the lists have a launch of their own."""
+    n, v = 900, 1031
+    x, ids, teacher, _ = make_distill(n, v, top, top, dtype)
+    weight = torch.ones(n, device="cuda")
+    x[0::9], weight[0::9] = math.nan, 0
+    ids[1::9] = -1
+    teacher[2::9] = -math.inf
+    x[3::9, ::2] = -math.inf
+    x[4::9] = -math.inf
+    x[5::9, 1:] = torch.finfo(dtype).min
+    ids[6::9] = 7
+    x[7::9, 20:] = -math.inf
+    ids[7::9] = ids[7::9] % 20
+    teacher[8::9, 1:] = -math.inf
+    loss, lse, grad = check_distill(T, x, ids, teacher, 1.0, weight)
+    assert not loss[0::9].any() and not grad[0::9].any() and not grad[1::9].any() and not grad[2::9].any() and bool((lse[4::9] == -math.inf).all())
+    assert bool(grad[4::9].isfinite().all())
 
 
 def test_distill_nan_stays_in_its_row(T):

@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 4) k_draw(const __grid_constant_
 //
 // With z = beta * logits, the row's softmax q = exp(z - lse) and the teacher's p over the listed entries:
 //     loss = sum_j p_j (log p_j - z_id(j) + lse),   d loss / d logits = beta (q - p).
-// Two kernels.  k_softmax streams the rows: lse (loss), weight * beta * q from a given lse (grad), or both (step), where the
+// Two kernels (one where rows are few).  k_softmax streams the rows: lse (loss), weight * beta * q from a given lse (grad), or both (step), where the
 // second pass finds the row in L2 (a CTA, or each of a cluster of up to eight, has 64 KB of it).  2048 x 131072 bf16: gradient
 // 152 us = 6.3 TB/s, the rate of a copy.  4096 x 32768 bf16: step 90 us = 5.3 TB/s.  k_listed then has one warp, or
 // four, for each row's list: the loss, and the few gradients that p changes.  What was measured and dropped (4096 x 32768 bf16,
@@ -678,9 +678,115 @@ struct Softmax {
     __device__ __forceinline__ float q(float l, float b2) const { return empty ? 0.0f : far ? far_weight(l, ref) * each : exp2_fast(fmaf(l, b2, shift)); }
 };
 
+// Slots of a list's table, a power of two: at most half of them are taken.
+__host__ __device__ inline int32_t list_slots(int32_t top) {
+    int32_t slots = 32;
+    while (slots < 2 * top) slots *= 2;
+    return slots;
+}
+
+// Shared memory of a row's list: ids, p, z and, for a gradient, the table and a bit per entry.
+__host__ __device__ inline int32_t list_words(int32_t top, int mode) { return 3 * top + (mode == LOSS ? 0 : list_slots(top) + (top + 31) / 32); }
+
+// A row's list, by a team of threads (`members`, whole warps, this thread number `me`; meet() is their barrier), whose arrays lie in
+// shared memory: the loss, and the gradient's listed entries among [low, high) once more, with p subtracted before the rounding.
+// sums() waits for the row's sums and gradient and gives its Softmax.  Categories that are listed more than once are found with a
+// table by open addressing (a step of 256 rows of 1024 entries 84 us; comparing all pairs 980).  The entry that got the slot
+// writes for all of them; which one that was changes nothing, as their sum is taken over the list in one order.
+template <class T, int MODE, class Meet, class Sums>
+__device__ __forceinline__ void finish_list(const DistillArgs& g, int64_t row, float weight, int32_t* id, int me, int members, bool tells, int32_t low, int32_t high, Meet meet, Sums sums) {
+    const int lane = threadIdx.x & 31;
+    float* p = reinterpret_cast<float*>(id + g.top);  // beta * teacher, then the softmax over the listed; id: -1 = not listed
+    float* z = p + g.top;                             // the student's logits there
+    int32_t* table = reinterpret_cast<int32_t*>(z + g.top);  // numbers of entries, -1 = free
+    const int32_t slots = list_slots(g.top);
+    uint32_t* more = reinterpret_cast<uint32_t*>(table + slots);  // bit j: entry j is not the only one of its category
+    uint32_t writes = 0;                                          // bit n: this thread's entry n writes for its category (32 at most)
+    const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
+    const float b2 = g.beta * LOG2E;
+    bool some = false;
+    float most = -INFINITY, total = 0.0f;
+    if (weight != 0.0f) {
+        if (MODE != LOSS)
+            for (int i = me; i < slots + (g.top + 31) / 32; i += members) table[i] = i < slots ? -1 : 0;
+#pragma unroll 4
+        for (int j = me; j < g.top; j += members) {
+            const int64_t k = load_as_int(g.ids, g.ids_type, row * g.ids_pitch + j);
+            const float t = g.beta * load_as_float(g.teacher, g.teacher_type, row * g.teacher_pitch + j);
+            const bool listed = k >= 0 && k < g.cols && !(t == -INFINITY);
+            id[j] = listed ? static_cast<int32_t>(k) : -1;
+            p[j] = t;
+            if (listed) z[j] = to_float(logits[k]);
+        }
+    }
+    meet();
+    if (weight != 0.0f) {
+        if (MODE != LOSS)
+            for (int j = me, n = 0; j < g.top; j += members, ++n) {
+                const int32_t k = id[j];
+                if (k < low || k >= high) continue;  // -1 among them
+                for (uint32_t at = static_cast<uint32_t>(k) * 2654435761u >> 16, tries = 0; tries < static_cast<uint32_t>(slots); ++at, ++tries) {
+                    const int32_t held = atomicCAS(table + (at & (slots - 1)), -1, j);
+                    if (held == -1) writes |= 1u << n;
+                    else if (id[held] == k) atomicOr(more + (held >> 5), 1u << (held & 31));
+                    else continue;
+                    break;
+                }
+            }
+        for (int j = lane; j < g.top; j += 32)
+            if (id[j] >= 0) {
+                most = fmaxf(most, p[j]);
+                some = true;
+            }
+        some = __any_sync(0xffffffffu, some);
+        most = warp_max(most);
+        for (int j = lane; j < g.top; j += 32) total += id[j] >= 0 ? expf(p[j] - most) : 0.0f;  // each warp of a team the same sum
+        total = warp_total(total);
+    }
+    meet();
+    if (weight != 0.0f)
+        for (int j = me; j < g.top; j += members) p[j] = id[j] >= 0 ? expf(p[j] - most) / total : 0.0f;
+    meet();
+    const Softmax soft = sums();
+    T* grad = MODE == LOSS ? nullptr : static_cast<T*>(g.grad) + row * g.grad_pitch;
+    if (weight == 0.0f || !some) {
+        if (MODE != GRAD && tells && me == 0) g.loss[row] = 0.0f, g.lse_out[row] = 0.0f;
+        if (MODE != LOSS && weight != 0.0f)
+            for (int32_t k = low + me; k < high; k += members) grad[k] = from_float<T>(0.0f);
+        return;
+    }
+    if (MODE != GRAD) {
+        meet();  // every thread has the row's sum, which may lie where the loss goes
+        if (tells && me < 32) {
+            const float log_sum = soft.sum2 * LN2;
+            float loss = 0.0f;
+            for (int j = lane; j < g.top; j += 32)
+                if (id[j] >= 0 && !(p[j] == 0.0f)) loss += soft.empty ? INFINITY : p[j] * (logf(p[j]) - g.beta * (z[j] - soft.ref) + log_sum);
+            loss = warp_total(loss);
+            if (lane == 0) g.loss[row] = loss;
+            if (lane == 0) g.lse_out[row] = soft.empty ? -INFINITY : fmaf(g.beta, soft.ref, log_sum);
+        }
+    }
+    if (MODE != LOSS)
+        for (int j = me, n = 0; j - lane < g.top; j += members, ++n) {  // whole warps
+            const bool mine = writes >> n & 1;
+            float share = mine ? p[j] : 0.0f;
+            for (unsigned several = __ballot_sync(0xffffffffu, mine && (more[j >> 5] >> (j & 31) & 1)); several; several &= several - 1) {
+                const int from = __ffs(several) - 1;
+                const int32_t k = id[j - lane + from];
+                float sum = 0.0f;
+                for (int t = lane; t < g.top; t += 32) sum += id[t] == k ? p[t] : 0.0f;
+                sum = warp_total(sum);
+                if (lane == from) share = sum;
+            }
+            if (mine) grad[id[j]] = from_float<T>(weight * g.beta * (soft.q(z[j], b2) - share));
+        }
+}
+
 // The rows' sums (reference into loss, log2 of the sum into lse_out, from where k_listed takes them), and weight * beta * q into
-// grad.
-template <class T, int MODE>
+// grad.  WHOLE: with few rows the list too, each CTA its own share's (a launch less: a step of 33 x 5003, 20 listed, 17.7 -> 14.6 us as
+// the host sees it, though 6.4 -> 7.0 on the GPU; 33 x 131072, 1024 listed, a gradient 42 -> 12 us).
+template <class T, int MODE, bool WHOLE>
 __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_constant__ DistillArgs g) {
     constexpr int V = VEC<T>, AT_ONCE = 4;
     __shared__ Partial warps[SOFTMAX_THREADS / 32], ctas[8];
@@ -688,7 +794,7 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
     const int64_t row = g.per_row == 1 ? blockIdx.x : blockIdx.x / g.per_row;
     const int32_t part = static_cast<int32_t>(blockIdx.x - row * g.per_row);
     const bool joined = MODE != GRAD && g.per_row > 1;  // the CTAs of a row form a cluster
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!WHOLE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (joined) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const float weight = g.weight ? g.weight[row] : 1.0f;  // 0: padding, nothing of the row is read
     const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
@@ -716,146 +822,73 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
             for (int c = 1; c < g.per_row; ++c) p.join(ctas[c], b2);
         }
         soft = Softmax::of(p, b2);
-        if (part == 0 && tid == 0) g.loss[row] = soft.ref, g.lse_out[row] = soft.sum2;
+        if (!WHOLE && part == 0 && tid == 0) g.loss[row] = soft.ref, g.lse_out[row] = soft.sum2;
     }
-    if (MODE == LOSS) return;
-    T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
-    const float scale = weight * g.beta;
-    const bool zeros = weight == 0.0f;
-    auto value = [&](float l) { return scale * soft.q(l, b2); };
-    if (tid < s.first - s.head) grad[s.head + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.head + tid])));
-    if (tid < s.stop - s.tail) grad[s.tail + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.tail + tid])));
-    if (((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15u) || soft.far) {
-        for (int32_t k = s.first + tid; k < s.tail; k += SOFTMAX_THREADS) grad[k] = from_float<T>(zeros ? 0.0f : value(to_float(logits[k])));
-        return;
-    }
-    uint4* out = reinterpret_cast<uint4*>(grad + s.first);
-    if (zeros) {
-        for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
-        return;
-    }
-    auto gradient = [&](const uint4& raw) {
-        float x[V];
-        unpack_16<T>(raw, x);
-#pragma unroll
-        for (int j = 0; j < V; j += 2) {
-            const float2 a = fma_2(make_float2(x[j], x[j + 1]), both(b2), both(soft.shift));
-            const float2 y = mul_2(make_float2(exp2_fast(a.x), exp2_fast(a.y)), both(scale));
-            x[j] = y.x, x[j + 1] = y.y;
+    auto write = [&] {
+        T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
+        const float scale = weight * g.beta;
+        const bool zeros = weight == 0.0f;
+        auto value = [&](float l) { return scale * soft.q(l, b2); };
+        if (tid < s.first - s.head) grad[s.head + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.head + tid])));
+        if (tid < s.stop - s.tail) grad[s.tail + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.tail + tid])));
+        if (((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15u) || soft.far) {
+            for (int32_t k = s.first + tid; k < s.tail; k += SOFTMAX_THREADS) grad[k] = from_float<T>(zeros ? 0.0f : value(to_float(logits[k])));
+            return;
         }
-        return pack_16<T>(x);
+        uint4* out = reinterpret_cast<uint4*>(grad + s.first);
+        if (zeros) {
+            for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
+            return;
+        }
+        auto gradient = [&](const uint4& raw) {
+            float x[V];
+            unpack_16<T>(raw, x);
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const float2 a = fma_2(make_float2(x[j], x[j + 1]), both(b2), both(soft.shift));
+                const float2 y = mul_2(make_float2(exp2_fast(a.x), exp2_fast(a.y)), both(scale));
+                x[j] = y.x, x[j + 1] = y.y;
+            }
+            return pack_16<T>(x);
+        };
+        int32_t i = tid;
+        for (; i + (AT_ONCE - 1) * SOFTMAX_THREADS < s.pieces; i += AT_ONCE * SOFTMAX_THREADS) {
+            uint4 raw[AT_ONCE];
+#pragma unroll
+            for (int t = 0; t < AT_ONCE; ++t) raw[t] = s.piece(i + t * SOFTMAX_THREADS);
+#pragma unroll
+            for (int t = 0; t < AT_ONCE; ++t) __stcs(out + i + t * SOFTMAX_THREADS, gradient(raw[t]));
+        }
+        for (; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, gradient(s.piece(i)));
     };
-    int32_t i = tid;
-    for (; i + (AT_ONCE - 1) * SOFTMAX_THREADS < s.pieces; i += AT_ONCE * SOFTMAX_THREADS) {
-        uint4 raw[AT_ONCE];
-#pragma unroll
-        for (int t = 0; t < AT_ONCE; ++t) raw[t] = s.piece(i + t * SOFTMAX_THREADS);
-#pragma unroll
-        for (int t = 0; t < AT_ONCE; ++t) __stcs(out + i + t * SOFTMAX_THREADS, gradient(raw[t]));
+    if (MODE != LOSS) write();
+    if (WHOLE) {
+        extern __shared__ int32_t listed_smem[];
+        __syncthreads();  // the share is written
+        finish_list<T, MODE>(g, row, weight, listed_smem, tid, SOFTMAX_THREADS, part == 0, s.head, s.stop, [] { __syncthreads(); }, [&] { return soft; });
     }
-    for (; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, gradient(s.piece(i)));
 }
 
-// The lists: a team of one warp per row, or of all LIST_WARPS where lists are long.  Reads lse, writes the loss, and writes the
-// gradient's listed entries once more, with p subtracted before the rounding.
+// The lists: a team of one warp per row, or of all LIST_WARPS where lists are long.  Everything up to the rows' sums is done while
+// k_softmax is still at work.
 template <class T, int MODE>
 __global__ void __launch_bounds__(32 * LIST_WARPS) k_listed(const __grid_constant__ DistillArgs g, int32_t teams) {
-    extern __shared__ int4 listed_smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int team = teams == 1 ? 0 : warp, members = teams == 1 ? blockDim.x : 32, me = teams == 1 ? threadIdx.x : lane;
+    extern __shared__ int32_t listed_smem[];
+    const int warp = threadIdx.x >> 5;
+    const int team = teams == 1 ? 0 : warp, members = teams == 1 ? blockDim.x : 32, me = teams == 1 ? threadIdx.x : threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team;
-    const bool here = row < g.rows;
+    if (row >= g.rows) return;  // a warp of its own
     auto meet = [&] {
         if (teams == 1) __syncthreads();
         else __syncwarp();
     };
-    const int top4 = (g.top + 3) & ~3;
-    int32_t* id = reinterpret_cast<int32_t*>(listed_smem) + 3 * top4 * team;  // -1 = not listed, up to a multiple of four
-    float* p = reinterpret_cast<float*>(id + top4);                           // beta * teacher, then the softmax over the listed
-    float* z = p + top4;                                                      // the student's logits there
-    const float weight = !here ? 0.0f : g.weight ? g.weight[row] : 1.0f;
-    const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
-    const float b2 = g.beta * LOG2E;
-    if (weight != 0.0f) {
-        if (me < top4 - g.top) id[g.top + me] = -1;
-#pragma unroll 4
-        for (int j = me; j < g.top; j += members) {
-            const int64_t k = load_as_int(g.ids, g.ids_type, row * g.ids_pitch + j);
-            const float t = g.beta * load_as_float(g.teacher, g.teacher_type, row * g.teacher_pitch + j);
-            const bool listed = k >= 0 && k < g.cols && !(t == -INFINITY);
-            id[j] = listed ? static_cast<int32_t>(k) : -1;
-            p[j] = t;
-            if (listed) z[j] = to_float(logits[k]);
-        }
-    }
-    meet();
-    bool some = false;
-    float most = -INFINITY, total = 0.0f;
-    if (weight != 0.0f) {
-        for (int j = lane; j < g.top; j += 32)
-            if (id[j] >= 0) {
-                most = fmaxf(most, p[j]);
-                some = true;
-            }
-        some = __any_sync(0xffffffffu, some);
-        most = warp_max(most);
-        for (int j = lane; j < g.top; j += 32) total += id[j] >= 0 ? expf(p[j] - most) : 0.0f;  // each warp of a team the same sum
-        total = warp_total(total);
-    }
-    meet();
-    if (weight != 0.0f)
-        for (int j = me; j < g.top; j += members) p[j] = id[j] >= 0 ? expf(p[j] - most) / total : 0.0f;
-    meet();
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows' sums and gradients
-    if (!here) return;
-    const bool counts = weight != 0.0f && some;
-    if (!counts) {
-        if (MODE != GRAD && me == 0) g.loss[row] = 0.0f;
-        if (MODE != GRAD && me == 0) g.lse_out[row] = 0.0f;
-        if (MODE != LOSS && weight != 0.0f) {
-            T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
-            for (int32_t k = me; k < g.cols; k += members) grad[k] = from_float<T>(0.0f);
-        }
-        return;
-    }
-    const Softmax soft = MODE == GRAD ? Softmax::of(g.lse_in[row], logits, g.cols, b2) : Softmax::of(g.loss[row], g.lse_out[row], b2);
-    if (MODE != GRAD) {
-        meet();  // every thread has read the row's sum before the loss takes its place
-        if (teams > 1 || warp == 0) {
-            const float log_sum = soft.sum2 * LN2;
-            float loss = 0.0f;
-            for (int j = lane; j < g.top; j += 32)
-                if (id[j] >= 0 && !(p[j] == 0.0f)) loss += soft.empty ? INFINITY : p[j] * (logf(p[j]) - g.beta * (z[j] - soft.ref) + log_sum);
-            loss = warp_total(loss);
-            if (lane == 0) g.loss[row] = loss;
-            if (lane == 0) g.lse_out[row] = soft.empty ? -INFINITY : fmaf(g.beta, soft.ref, log_sum);
-        }
-    }
-    if (MODE != LOSS) {
-        T* grad = static_cast<T*>(g.grad) + row * g.grad_pitch;
-        for (int j = me; j < g.top; j += members) {
-            const int32_t k = id[j];
-            if (k < 0) continue;
-            // the first entry of a category that is listed more than once writes for all of them
-            int same = 0;
-#pragma unroll 4
-            for (int i = 0; i < g.top; i += 4) {
-                const int4 o = *reinterpret_cast<const int4*>(id + i);
-                same += (o.x == k) + (o.y == k) + (o.z == k) + (o.w == k);
-            }
-            float share = p[j];
-            bool first = true;
-            if (same > 1) {
-                share = 0.0f;
-                for (int i = 0; i < g.top; ++i)
-                    if (id[i] == k) {
-                        first &= i >= j;
-                        share += p[i];
-                    }
-            }
-            if (first) grad[k] = from_float<T>(weight * g.beta * (soft.q(z[j], b2) - share));
-        }
-    }
+    auto sums = [&] {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const float b2 = g.beta * LOG2E;
+        return MODE == GRAD ? Softmax::of(g.lse_in[row], static_cast<const T*>(g.logits) + row * g.pitch, g.cols, b2) : Softmax::of(g.loss[row], g.lse_out[row], b2);
+    };
+    int32_t* arrays = listed_smem + list_words(g.top, MODE) * team;
+    finish_list<T, MODE>(g, row, g.weight ? g.weight[row] : 1.0f, arrays, me, members, true, 0, g.cols, meet, sums);
 }
 
 // Positions of a row, counted from the last 16-byte boundary at or before it (the most that any row has).
@@ -895,12 +928,18 @@ int32_t launch_distill(thrml_ctx* ctx, cudaStream_t stream, DistillArgs g) {
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {static_cast<unsigned>(per_row), 1, 1};
     cfg.numAttrs = MODE != GRAD && per_row > 1 ? 1 : 0;
-    CU_TRY(cudaLaunchKernelEx(&cfg, k_softmax<T, MODE>, g));
+    const size_t list_bytes = 4 * static_cast<size_t>(list_words(g.top, MODE));
+    if (g.rows * per_row <= 2 * ctx->sm_count) {
+        cfg.dynamicSmemBytes = list_bytes;
+        CU_TRY(cudaLaunchKernelEx(&cfg, k_softmax<T, MODE, true>, g));
+        return THRML_OK;
+    }
+    CU_TRY(cudaLaunchKernelEx(&cfg, k_softmax<T, MODE, false>, g));
     // The lists start while the last rows are still at work; what they need of those they wait for.
-    const int32_t teams = g.top <= 64 ? LIST_WARPS : 1;  // a warp for 64 entries; four for 128 save 10 us of 184 (gradient, 2048 x 131072)
+    const int32_t teams = g.top <= 64 ? LIST_WARPS : 1;  // a warp for 64 entries; four for 128 save 7 us of 188 (gradient, 2048 x 131072)
     cfg.gridDim = dim3(static_cast<unsigned>((g.rows + teams - 1) / teams));
     cfg.blockDim = dim3(32 * LIST_WARPS);
-    cfg.dynamicSmemBytes = 12 * static_cast<size_t>((g.top + 3) / 4 * 4) * teams;
+    cfg.dynamicSmemBytes = list_bytes * teams;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
