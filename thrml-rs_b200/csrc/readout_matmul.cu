@@ -30,9 +30,11 @@ __device__ __forceinline__ int32_t quantise(float x, float scale, float inverse)
     return static_cast<int32_t>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
-// Bound by memory.  A CTA has a row: as many threads as hold it in four 16-byte pieces each (32 to 256; a longer row's rest is
-// read a second time), in registers between the maximum and the quotients.
-constexpr int QUANT_THREADS = 256, QUANT_PIECES = 4;
+// Bound by memory.  A CTA has a row: as many threads as hold it in two 16-byte pieces each (32 to 512; a longer row's rest is
+// read a second time), in registers between the maximum and the quotients.  Four pieces and 256 threads are no faster on rows of 4096
+// (2048 of them, bf16: 11 us against 10.5) and slower on long ones (256 of 131072: 53 against 32); 1024 threads 2048 of 16384: 53
+// against 34.
+constexpr int QUANT_THREADS = 512, QUANT_PIECES = 2;
 
 // A row's scale, from the largest magnitude in it.
 struct Scale {
