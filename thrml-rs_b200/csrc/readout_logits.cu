@@ -41,9 +41,11 @@ __device__ __forceinline__ uint4 nothing_16() {
 // ---------------------------------------------------------------------------------------------------------
 // Rules on logits.
 //
-// Bound by memory: every logit is read and written once.  A CTA copies a share of a row into shared memory, ADJUST_PIECES 16-byte
-// pieces a thread, in flight together; meanwhile it counts there those of the row's tokens that fall into the share (integer atomics, so the counts do not depend on their order).  A count has 16 bits, and 32 in rows of 2^15 tokens
-// or more, which are done half a share at a time.  Every CTA of a row reads the whole history, from L2 after the first.
+// Every logit is read and written once.  A CTA copies a share of a row into shared memory, ADJUST_PIECES 16-byte pieces a thread,
+// in flight together; meanwhile it counts there those of the row's tokens that fall into the share (integer atomics, so the counts
+// do not depend on their order).  A count has 16 bits, and 32 in rows of 2^15 tokens or more, which are done half a share at a time.
+// Every CTA of a row reads the whole history, from L2 after the first.  256 x 131072 bf16 with 4096 tokens, biases and masks 56 us =
+// 2.4 TB/s, bound by instruction issue; without any rule 23, by memory.
 // Categories with a bias are finished by a thread of their own, before the pass over the share, which leaves out what a bitmap
 // marks.  Measured and dropped for 256 rows of 131072 bf16 with 3000 tokens each: the few named categories in a kernel of
 // their own behind a plain copy, 77 us (their scattered 2-byte writes cost more than they are); for 16 rows with 60000
