@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
 // (where two scores that f32 cannot tell apart have an order), which decides.  B starts from approximate scores of each
 // thread's first categories, lowered by more than their error, and rises with the scores found, shared in the CTA.
 // Bound by instruction issue: ten rounds of the generator serve four categories.  256 x 131072 bf16: 52 us with two CTAs a
-// row, 60 with four and 75 with eight, whose starts and first, loose bounds cost more than they spread.
+// row, 60 with four and 75 with eight, whose starts and first, loose bounds cost more than they spread.  Four CTAs of 128
+// threads, which spread evenly over the SMs: 56; 512 x 32000 38 instead of 33, though 2048 x 5003 34 instead of 40.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int DRAW_THREADS = 256, DRAW_GROUP = 8;  // categories that share two generator calls
 constexpr int DRAW_AT_ONCE = 2;                     // groups of a thread whose logits are in flight together
