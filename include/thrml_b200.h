@@ -579,10 +579,10 @@ int32_t thrml_draw_categories(thrml_ctx* ctx, void* stream, int64_t rows, int64_
  * entries whose id lies outside [0, cols) or whose logit is -infinity are not listed, a category listed twice counts twice.
  *   p = softmax over the listed of beta * teacher,  q = softmax over all categories of beta * logits,
  *   loss[r] = sum_j p_j (log p_j - log q_id(j)),    grad[r][k] = weight[r] * beta * (q_k - p_k)   (p_k summed over entries)
- * = weight[r] times the derivative of loss[r] by logits[r][k]; weight NULL = 1; beta > 0, finite.  A row of weight 0 (padding) is not
+ * = weight[r] times the derivative of loss[r] by logits[r][k]; weight NULL = 1; beta within 2^-100 and 2^100.  A row of weight 0 (padding) is not
  * read: its loss and gradient are 0.  A row that lists nothing likewise.  A row of logits that are all -infinity has q = 0 and
  * loss = infinity.  lse[r] = log sum_k exp(beta * logits[r][k]) (0 where loss and gradient are 0 as said); thrml_distill_grad takes
- * it back from thrml_distill_loss; thrml_distill_step gives loss and gradient with the weights known beforehand, reading the
+ * it back from thrml_distill_loss, and forms the sums of a row of |lse| above 256, which lse holds too coarsely, again; thrml_distill_step gives loss and gradient with the weights known beforehand, reading the
  * logits once from memory.  grad has the logits' type and does not overlap them. */
 int32_t thrml_distill_loss(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, int64_t top, const void* ids,
                            int32_t ids_type, int64_t ids_pitch, const void* teacher, int32_t teacher_type, int64_t teacher_pitch, float beta, const float* weight,

@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 4) k_draw(const __grid_constant_
 // 64 listed, a step): rows held in registers or in shared memory, once per CTA or in rings of two and three rows, the
 // list inside the same kernel: 125 to 200 us, since the list's chain of small loads, each as slow as a full memory system
 // makes it, held up the rows.
-// Per element one multiply-add and one hardware exponential a pass, in base 2, two elements an instruction where there is
+// Per element a difference, a product or multiply-add and one hardware exponential a pass, in base 2, two elements an instruction where there is
 // one; probabilities below 2^-126 count as 0.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int SOFTMAX_THREADS = 256;
@@ -516,29 +516,23 @@ struct DistillArgs {
     int32_t share, per_row;  // positions of a row per CTA, CTAs per row
 };
 
-// Where beta times the largest logit is FAR or more, neighbouring values of the type lie so far apart that a category either
-// is the largest or has no weight; there (rows whose mask is the type's lowest value and leaves nothing) the scaled logits could
-// overflow, and are not formed.
-constexpr float FAR = 0x1p100f;
-__device__ __forceinline__ bool is_far(float z) { return !(fabsf(z) < FAR); }
-__device__ __forceinline__ float far_weight(float l, float most) { return l != l ? l : l == most ? (most == INFINITY ? NAN : most == -INFINITY ? 0.0f : 1.0f) : 0.0f; }
+// beta's range: a finite difference of two logits that f32 cannot hold is then weight 0, and base 2 does not overflow.
+constexpr float BETA_MIN = 0x1p-100f, BETA_MAX = 0x1p100f;
+// The largest |lse| that a gradient takes as it is: its rounding is a relative error of q of up to 2^-17 there and grows with it, so
+// the sums of a row beyond (a mask's fill that leaves nothing, mostly) are formed again, which costs another reading of the row.
+constexpr float LSE_KEPT = 256.0f;
 
-// A part of a softmax's sum: 2^(b2 l - b2 ref) over its logits l, with b2 ref rounded.  ref is one of the logits or above them,
-// the largest where it is far; -infinity while there is nothing.
+// A part of a softmax's sum: 2^(b2 (l - ref)) over its logits l.  ref is one of them, -infinity while there is nothing.  The
+// difference comes first: it is exact next to ref, however large both are, where rounded products would lie apart.
 struct Partial {
     float ref, sum;
     __device__ __forceinline__ void join(Partial o, float b2) {
         const float top = fmaxf(ref, o.ref);
         // a part at -infinity adds nothing; its sum is 0, or NaN when it has met one
-        const float a = ref == top || ref == -INFINITY ? 1.0f : step(ref, top, b2);
-        const float b = o.ref == top || o.ref == -INFINITY ? 1.0f : step(o.ref, top, b2);
+        const float a = ref == top || ref == -INFINITY ? 1.0f : exp2_fast((ref - top) * b2);
+        const float b = o.ref == top || o.ref == -INFINITY ? 1.0f : exp2_fast((o.ref - top) * b2);
         sum = fmaf(sum, a, o.sum * b);
         ref = top;
-    }
-    // From one rounded b2 ref to the other; differences first where the products could overflow (the result is 0 there).
-    static __device__ __forceinline__ float step(float from, float to, float b2) {
-        const float a = __fmul_rn(from, b2), b = __fmul_rn(to, b2);
-        return exp2_fast(fabsf(a) < INFINITY && fabsf(b) < INFINITY ? a - b : (from - to) * b2);
     }
 };
 
@@ -572,21 +566,19 @@ __device__ __forceinline__ float warp_total(float x) {
     return x;
 }
 
-// A warp's part of the share's sum: with the maximum of its logits first.
-template <class T>
-__device__ __noinline__ Partial sum_carefully(const Share<T>& s, float b2) {
-    const int tid = threadIdx.x;
+// A warp's part of the share's sum, the share being dealt to THREADS threads: with the maximum of its logits first.
+template <class T, int THREADS>
+__device__ __noinline__ Partial sum_carefully(const Share<T>& s, float b2, int tid) {
     float high = -INFINITY, other = -INFINITY;
-    for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) larger_16<T>(high, other, s.piece(i));
+    for (int32_t i = tid; i < s.pieces; i += THREADS) larger_16<T>(high, other, s.piece(i));
     high = fmaxf(upper<T>(high), other);
     if (s.head + tid < s.first) high = fmaxf(high, to_float(s.row[s.head + tid]));
     if (s.tail + tid < s.stop) high = fmaxf(high, to_float(s.row[s.tail + tid]));
     high = warp_max(high);
     const float low = high == -INFINITY ? 0.0f : high;
-    const bool far = is_far(low * b2);
-    auto weight = [&](float l) { return far ? far_weight(l, low) : exp2_fast(fmaf(l, b2, -low * b2)); };
+    auto weight = [&](float l) { return exp2_fast((l - low) * b2); };
     float sum = 0.0f;
-    for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) {
+    for (int32_t i = tid; i < s.pieces; i += THREADS) {
         float v[VEC<T>];
         unpack_16<T>(s.piece(i), v);
 #pragma unroll
@@ -596,89 +588,70 @@ __device__ __noinline__ Partial sum_carefully(const Share<T>& s, float b2) {
     if (s.tail + tid < s.stop) sum += weight(to_float(s.row[s.tail + tid]));
     return Partial{high, warp_total(sum)};
 }
-template <class T>
-__device__ __forceinline__ Partial sum_of(const Share<T>& s, float b2) {
+template <class T, int THREADS>
+__device__ __forceinline__ Partial sum_of(const Share<T>& s, float b2, int tid) {
     constexpr int V = VEC<T>, AT_ONCE = 4;
-    const int tid = threadIdx.x;
     // The reference is the largest of the warp's first pieces, which spares a pass for the maximum: sums are good as long as they
     // stay below 2^100, and what does not is done over with the maximum.
     float2 sums = both(0.0f), more = both(0.0f);
     float ref = -INFINITY, other = -INFINITY;
     if (tid < s.pieces) larger_16<T>(ref, other, s.piece(tid));
     ref = warp_max(fmaxf(upper<T>(ref), other));
-    const float2 scale = both(b2), shift = both(-ref * b2);
+    const float2 scale = both(b2), back = both(-ref);
     auto add = [&](const uint4& raw) {
         float v[V];
         unpack_16<T>(raw, v);
 #pragma unroll
         for (int j = 0; j < V; j += 4) {
-            const float2 a = fma_2(make_float2(v[j], v[j + 1]), scale, shift), b = fma_2(make_float2(v[j + 2], v[j + 3]), scale, shift);
+            const float2 a = mul_2(add_2(make_float2(v[j], v[j + 1]), back), scale), b = mul_2(add_2(make_float2(v[j + 2], v[j + 3]), back), scale);
             sums = add_2(sums, make_float2(exp2_fast(a.x), exp2_fast(a.y)));
             more = add_2(more, make_float2(exp2_fast(b.x), exp2_fast(b.y)));
         }
     };
     int32_t i = tid;
-    for (; i + (AT_ONCE - 1) * SOFTMAX_THREADS < s.pieces; i += AT_ONCE * SOFTMAX_THREADS) {
+    for (; i + (AT_ONCE - 1) * THREADS < s.pieces; i += AT_ONCE * THREADS) {
         uint4 raw[AT_ONCE];
 #pragma unroll
-        for (int t = 0; t < AT_ONCE; ++t) raw[t] = s.piece(i + t * SOFTMAX_THREADS);
+        for (int t = 0; t < AT_ONCE; ++t) raw[t] = s.piece(i + t * THREADS);
 #pragma unroll
         for (int t = 0; t < AT_ONCE; ++t) add(raw[t]);
     }
-    for (; i < s.pieces; i += SOFTMAX_THREADS) add(s.piece(i));
+    for (; i < s.pieces; i += THREADS) add(s.piece(i));
     float sum = (sums.x + sums.y) + (more.x + more.y);
-    if (s.head + tid < s.first) sum += exp2_fast(fmaf(to_float(s.row[s.head + tid]), b2, shift.x));
-    if (s.tail + tid < s.stop) sum += exp2_fast(fmaf(to_float(s.row[s.tail + tid]), b2, shift.x));
+    if (s.head + tid < s.first) sum += exp2_fast((to_float(s.row[s.head + tid]) - ref) * b2);
+    if (s.tail + tid < s.stop) sum += exp2_fast((to_float(s.row[s.tail + tid]) - ref) * b2);
     sum = warp_total(sum);
-    if (!(sum < 0x1p100f) || is_far(ref * b2)) return sum_carefully(s, b2);
+    if (!(sum < 0x1p100f)) return sum_carefully<T, THREADS>(s, b2, tid);  // an infinite reference among them
     return Partial{ref, sum};
 }
-
-// The row's largest logit and the number of categories that share it, by every warp for itself (far rows of which only lse is
-// known).
-template <class T>
-__device__ __noinline__ Partial count_largest(const T* logits, int32_t cols) {
-    const int lane = threadIdx.x & 31;
-    float high = -INFINITY, n = 0.0f;
-    for (int32_t k = lane; k < cols; k += 32) high = fmaxf(high, to_float(logits[k]));
-    high = warp_max(high);
-    for (int32_t k = lane; k < cols; k += 32) n += far_weight(to_float(logits[k]), high);
-    return Partial{high, warp_total(n)};
+// The sum of a whole row, by a CTA of THREADS threads or a warp (rows whose lse a gradient does not take as it is).
+template <class T, int THREADS>
+__device__ __noinline__ Partial sum_again(const T* logits, int32_t cols, float b2, int tid, Partial* warps) {
+    Partial p = sum_of<T, THREADS>(Share<T>(logits, cols, 0, cols + VEC<T>), b2, tid);
+    if (THREADS > 32) {
+        if ((tid & 31) == 0) warps[tid >> 5] = p;
+        __syncthreads();
+        p = warps[0];
+        for (int w = 1; w < THREADS / 32; ++w) p.join(warps[w], b2);
+    }
+    return p;
 }
 
-// q of a row, from the joined parts of its sum or from its lse.
+// q of a row, from the joined parts of its sum or from its lse: 2^(b2 (l - ref) - sum2).
 struct Softmax {
-    float ref, sum2;  // a logit, and log2 of the sum relative to it
-    float shift, each;
-    bool far, empty;
-    __device__ __forceinline__ static Softmax of(Partial p, float b2) {
-        Softmax s;
-        s.ref = p.ref;
-        s.far = is_far(p.ref * b2);
-        s.empty = p.ref == -INFINITY && p.sum == 0.0f;
-        s.sum2 = p.sum == INFINITY || (p.ref == -INFINITY && p.sum != 0.0f) ? NAN : log2f(p.sum);
-        if (!s.far) s.sum2 += fmaf(-p.ref, b2, __fmul_rn(p.ref, b2));  // relative to b2 ref itself
-        s.finish(b2);
-        return s;
+    float ref, sum2;  // a logit, or a number near one, and log2 of the sum relative to it
+    bool empty;
+    __device__ __forceinline__ static Softmax of(Partial p) { return of(p.ref, p.sum == INFINITY || (p.ref == -INFINITY && p.sum != 0.0f) ? NAN : log2f(p.sum)); }
+    __device__ __forceinline__ static Softmax of(float ref, float sum2) { return Softmax{ref, sum2, ref == -INFINITY && sum2 == -INFINITY}; }
+    // lse as beta ref + a rest, so that here too the difference comes first.
+    __device__ __forceinline__ static Softmax of_lse(float lse, float beta) {
+        const float ref = lse / beta;
+        return Softmax{ref, LOG2E * static_cast<float>(lse - static_cast<double>(beta) * ref), false};
     }
-    __device__ __forceinline__ static Softmax of(float ref, float sum2, float b2) {
-        Softmax s;
-        s.ref = ref, s.sum2 = sum2;
-        s.far = is_far(ref * b2);
-        s.empty = ref == -INFINITY && sum2 == -INFINITY;
-        s.finish(b2);
-        return s;
-    }
-    template <class T>
-    __device__ __forceinline__ static Softmax of(float lse, const T* logits, int32_t cols, float b2) {
-        if (lse == lse && is_far(lse)) return of(count_largest(logits, cols), b2);  // so far out lse cannot say how many share the weight
-        return of(0.0f, lse * LOG2E, b2);
-    }
-    __device__ __forceinline__ void finish(float b2) {
-        each = far ? exp2_fast(-sum2) : 0.0f;
-        shift = fmaf(-ref, b2, -sum2);
-    }
-    __device__ __forceinline__ float q(float l, float b2) const { return empty ? 0.0f : far ? far_weight(l, ref) * each : exp2_fast(fmaf(l, b2, shift)); }
+    // What is taken from a logit, and from the exponent: a row with nothing has q = 0.
+    __device__ __forceinline__ float back() const { return empty ? 0.0f : ref; }
+    __device__ __forceinline__ float less() const { return empty ? INFINITY : sum2; }
+    __device__ __forceinline__ float q(float l, float b2) const { return exp2_fast(fmaf(l - back(), b2, -less())); }
 };
 
 // Slots of a list's table, a power of two: at most half of them are taken.
@@ -764,7 +737,10 @@ __device__ __forceinline__ void finish_list(const DistillArgs& g, int64_t row, f
             const float log_sum = soft.sum2 * LN2;
             float loss = 0.0f;
             for (int j = lane; j < g.top; j += 32)
-                if (id[j] >= 0 && !(p[j] == 0.0f)) loss += soft.empty ? INFINITY : p[j] * (logf(p[j]) - g.beta * (z[j] - soft.ref) + log_sum);
+                if (id[j] >= 0 && !(p[j] == 0.0f)) {
+                    const float gap = fmaf(-0.5f, soft.ref, 0.5f * z[j]);  // half of the difference, which f32 may not hold
+                    loss += soft.empty ? INFINITY : p[j] * (logf(p[j]) + log_sum) + (gap == -INFINITY ? INFINITY : -2.0f * p[j] * g.beta * gap);
+                }
             loss = warp_total(loss);
             if (lane == 0) g.loss[row] = loss;
             if (lane == 0) g.lse_out[row] = soft.empty ? -INFINITY : fmaf(g.beta, soft.ref, log_sum);
@@ -805,10 +781,13 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
     const float b2 = g.beta * LOG2E;
     Softmax soft{};
     if (MODE == GRAD) {
-        if (weight != 0.0f) soft = Softmax::of(g.lse_in[row], logits, g.cols, b2);
+        if (weight != 0.0f) {
+            const float lse = g.lse_in[row];
+            soft = fabsf(lse) > LSE_KEPT ? Softmax::of(sum_again<T, SOFTMAX_THREADS>(logits, g.cols, b2, tid, warps)) : Softmax::of_lse(lse, g.beta);
+        }
     } else {
         Partial p{-INFINITY, 0.0f};
-        if (weight != 0.0f) p = sum_of(s, b2);
+        if (weight != 0.0f) p = sum_of<T, SOFTMAX_THREADS>(s, b2, tid);
         if (lane == 0) warps[tid >> 5] = p;
         __syncthreads();
         p = warps[lane & (SOFTMAX_THREADS / 32 - 1)];
@@ -824,7 +803,7 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
             p = ctas[0];
             for (int c = 1; c < g.per_row; ++c) p.join(ctas[c], b2);
         }
-        soft = Softmax::of(p, b2);
+        soft = Softmax::of(p);
         if (!WHOLE && part == 0 && tid == 0) g.loss[row] = soft.ref, g.lse_out[row] = soft.sum2;
     }
     auto write = [&] {
@@ -834,7 +813,7 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
         auto value = [&](float l) { return scale * soft.q(l, b2); };
         if (tid < s.first - s.head) grad[s.head + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.head + tid])));
         if (tid < s.stop - s.tail) grad[s.tail + tid] = from_float<T>(zeros ? 0.0f : value(to_float(logits[s.tail + tid])));
-        if (((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15u) || soft.far) {
+        if ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(logits)) & 15u) {
             for (int32_t k = s.first + tid; k < s.tail; k += SOFTMAX_THREADS) grad[k] = from_float<T>(zeros ? 0.0f : value(to_float(logits[k])));
             return;
         }
@@ -843,12 +822,13 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
             for (int32_t i = tid; i < s.pieces; i += SOFTMAX_THREADS) __stcs(out + i, make_uint4(0u, 0u, 0u, 0u));
             return;
         }
+        const float2 back = both(-soft.back()), less = both(-soft.less());
         auto gradient = [&](const uint4& raw) {
             float x[V];
             unpack_16<T>(raw, x);
 #pragma unroll
             for (int j = 0; j < V; j += 2) {
-                const float2 a = fma_2(make_float2(x[j], x[j + 1]), both(b2), both(soft.shift));
+                const float2 a = fma_2(add_2(make_float2(x[j], x[j + 1]), back), both(b2), less);
                 const float2 y = mul_2(make_float2(exp2_fast(a.x), exp2_fast(a.y)), both(scale));
                 x[j] = y.x, x[j + 1] = y.y;
             }
@@ -877,6 +857,7 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
 template <class T, int MODE>
 __global__ void __launch_bounds__(32 * LIST_WARPS) k_listed(const __grid_constant__ DistillArgs g, int32_t teams) {
     extern __shared__ int32_t listed_smem[];
+    __shared__ Partial warps[LIST_WARPS];
     const int warp = threadIdx.x >> 5;
     const int team = teams == 1 ? 0 : warp, members = teams == 1 ? blockDim.x : 32, me = teams == 1 ? threadIdx.x : threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * teams + team;
@@ -885,13 +866,18 @@ __global__ void __launch_bounds__(32 * LIST_WARPS) k_listed(const __grid_constan
         if (teams == 1) __syncthreads();
         else __syncwarp();
     };
+    const float weight = g.weight ? g.weight[row] : 1.0f;
     auto sums = [&] {
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        const float b2 = g.beta * LOG2E;
-        return MODE == GRAD ? Softmax::of(g.lse_in[row], static_cast<const T*>(g.logits) + row * g.pitch, g.cols, b2) : Softmax::of(g.loss[row], g.lse_out[row], b2);
+        if (weight == 0.0f) return Softmax{};
+        if (MODE != GRAD) return Softmax::of(g.loss[row], g.lse_out[row]);
+        const float lse = g.lse_in[row], b2 = g.beta * LOG2E;
+        if (!(fabsf(lse) > LSE_KEPT)) return Softmax::of_lse(lse, g.beta);
+        const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
+        return Softmax::of(teams == 1 ? sum_again<T, 32 * LIST_WARPS>(logits, g.cols, b2, me, warps) : sum_again<T, 32>(logits, g.cols, b2, me, warps));
     };
     int32_t* arrays = listed_smem + list_words(g.top, MODE) * team;
-    finish_list<T, MODE>(g, row, g.weight ? g.weight[row] : 1.0f, arrays, me, members, true, 0, g.cols, meet, sums);
+    finish_list<T, MODE>(g, row, weight, arrays, me, members, true, 0, g.cols, meet, sums);
 }
 
 // Positions of a row, counted from the last 16-byte boundary at or before it (the most that any row has).
@@ -960,7 +946,7 @@ int32_t distill(thrml_ctx* ctx, void* stream, int mode, int64_t rows, int32_t ty
     if (!is_index_type(g.ids_type)) return fail(THRML_ERR_INVALID_ARG, "ids: the element type is not an index type");
     if (!is_float_type(g.teacher_type)) return fail(THRML_ERR_INVALID_ARG, "teacher: the element type is not a float type");
     if (g.ids_pitch < g.top || g.teacher_pitch < g.top) return fail(THRML_ERR_INVALID_ARG, "ids, teacher: the pitch is smaller than top");
-    if (!(g.beta > 0.0f) || g.beta == INFINITY) return fail(THRML_ERR_INVALID_ARG, "beta has to be positive and finite");
+    if (!(g.beta >= BETA_MIN && g.beta <= BETA_MAX)) return fail(THRML_ERR_INVALID_ARG, "beta is not within 2^-100 and 2^100");
     if (rows == 0) return THRML_OK;
     if (g.top && (!g.ids || !g.teacher)) return fail(THRML_ERR_INVALID_ARG, "ids, teacher: null pointer");
     if ((mode != GRAD && !g.loss) || (mode != GRAD && !g.lse_out) || (mode == GRAD && !g.lse_in)) return fail(THRML_ERR_INVALID_ARG, "loss, lse: null pointer");
