@@ -130,3 +130,18 @@ def test_distill_padding_has_no_lse(T, times):
     lse[:, 1], lse[:, 2], lse[:, 3] = math.nan, math.inf, 1e30
     x.view(times, 4, -1)[:, 1:] = math.nan
     assert torch.equal(T.distill_grad(x, lse.reshape(-1), ids, teacher, weight=weight), want) and not want.view(times, 4, -1)[:, 1:].any()
+
+
+@pytest.mark.parametrize("beta", [0.5, 0.7, 1.0, 2.0])
+@pytest.mark.parametrize("times", [1, 120])
+def test_distill_large_teacher_logits(T, beta, times):
+    """The teacher's logits likewise: entries a few steps apart at any size, and a list that is all the lowest value."""
+    n = 3000
+    x = torch.randn(4, n, generator=gen(1), device="cuda")
+    ids = torch.arange(9, device="cuda")[None].repeat(4, 1) * 7
+    for size in SIZES + [torch.finfo(torch.float32).max]:
+        t = torch.full((4, 9), -size, device="cuda")
+        t[1] = size * (1 - 2 * half(torch.float32) * torch.arange(9, device="cuda"))
+        t[2, ::2] = size
+        t[3] = -t[1]
+        check_large(T, x, ids, t, beta, times)

@@ -672,7 +672,7 @@ __host__ __device__ inline int32_t list_words(int32_t top, int mode) { return 3 
 template <class T, int MODE, class Meet, class Sums>
 __device__ __forceinline__ void finish_list(const DistillArgs& g, int64_t row, float weight, int32_t* id, int me, int members, bool tells, int32_t low, int32_t high, Meet meet, Sums sums) {
     const int lane = threadIdx.x & 31;
-    float* p = reinterpret_cast<float*>(id + g.top);  // beta * teacher, then the softmax over the listed; id: -1 = not listed
+    float* p = reinterpret_cast<float*>(id + g.top);  // the teacher's logits, then their softmax over the listed (differences first, as in Partial); id: -1 = not listed
     float* z = p + g.top;                             // the student's logits there
     int32_t* table = reinterpret_cast<int32_t*>(z + g.top);  // numbers of entries, -1 = free
     const int32_t slots = list_slots(g.top);
@@ -688,7 +688,7 @@ __device__ __forceinline__ void finish_list(const DistillArgs& g, int64_t row, f
 #pragma unroll 4
         for (int j = me; j < g.top; j += members) {
             const int64_t k = load_as_int(g.ids, g.ids_type, row * g.ids_pitch + j);
-            const float t = g.beta * load_as_float(g.teacher, g.teacher_type, row * g.teacher_pitch + j);
+            const float t = load_as_float(g.teacher, g.teacher_type, row * g.teacher_pitch + j);
             const bool listed = k >= 0 && k < g.cols && !(t == -INFINITY);
             id[j] = listed ? static_cast<int32_t>(k) : -1;
             p[j] = t;
@@ -716,12 +716,12 @@ __device__ __forceinline__ void finish_list(const DistillArgs& g, int64_t row, f
             }
         some = __any_sync(0xffffffffu, some);
         most = warp_max(most);
-        for (int j = lane; j < g.top; j += 32) total += id[j] >= 0 ? expf(p[j] - most) : 0.0f;  // each warp of a team the same sum
+        for (int j = lane; j < g.top; j += 32) total += id[j] >= 0 ? expf(g.beta * (p[j] - most)) : 0.0f;  // each warp of a team the same sum
         total = warp_total(total);
     }
     meet();
     if (weight != 0.0f)
-        for (int j = me; j < g.top; j += members) p[j] = id[j] >= 0 ? expf(p[j] - most) / total : 0.0f;
+        for (int j = me; j < g.top; j += members) p[j] = id[j] >= 0 ? expf(g.beta * (p[j] - most)) / total : 0.0f;
     meet();
     const Softmax soft = sums();
     T* grad = MODE == LOSS ? nullptr : static_cast<T*>(g.grad) + row * g.grad_pitch;
