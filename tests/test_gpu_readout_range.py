@@ -145,3 +145,19 @@ def test_distill_large_teacher_logits(T, beta, times):
         t[2, ::2] = size
         t[3] = -t[1]
         check_large(T, x, ids, t, beta, times)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("beta", [1e30, 1e38, 2.3e38, 2.4e38, torch.finfo(torch.float32).max])
+@pytest.mark.parametrize("r, v", [(3, 5), (4, 3001), (2, 131072), (700, 40)])
+def test_draw_categories_large_beta(T, dtype, beta, r, v):
+    """Temperatures next to 0: the largest logit wins, among log-probabilities, positive logits and both; -infinity is masked."""
+    x = torch.randn(r, v, generator=gen(v), device="cuda") * 3
+    x[0] = x[0].log_softmax(0)  # every product with beta may overflow, or none
+    x[-1] = x[-1].abs().neg() * 0.1
+    x[1, ::3] = -math.inf
+    x = x.to(dtype)
+    b = torch.full((r,), beta, device="cuda")
+    assert torch.equal(T.draw_categories(x, 77, beta=b).cpu(), draw64(x, uniforms(r, v, 77), b))
+    noise = torch.rand(r, v, generator=gen(9), device="cuda").clamp_(1e-6, 0.999999)
+    assert torch.equal(T.draw_categories(x, 77, beta=b, noise=noise).cpu(), draw64(x, noise.cpu().numpy(), b))

@@ -395,6 +395,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 4) k_draw(const __grid_constant_
             for (int j = 0; j < DRAW_GROUP; ++j) some |= l[j] >= b;
             return some;
         }
+        if (b2 == INFINITY) return true;  // a beta near the largest f32: base 2 cannot hold it, and weigh() decides
 #pragma unroll
         for (int h = 0; h < DRAW_GROUP; h += 4) {
             float f[4];
