@@ -161,6 +161,9 @@ int32_t thrml_greedy_coloring_device(thrml_ctx* ctx, int64_t n_nodes, int64_t n_
  * kernel waits on a pipeline barrier that nothing signals; its bounded wait runs out, it returns, and this call
  * reports THRML_ERR_TIMEOUT.  The context remains usable. */
 int32_t thrml_debug_wait_timeout(thrml_ctx* ctx);
+/* The same for the categorical readout's report, asynchronously on the caller's stream: the wait runs out there, and from then on the
+ * context's readout calls and thrml_ctx_synchronize return THRML_ERR_TIMEOUT until thrml_ctx_reset_waits. */
+int32_t thrml_debug_lose_wait(thrml_ctx* ctx, void* stream);
 /* cudaStream_t of the context, for callers that time with their own events. */
 void* thrml_ctx_stream(thrml_ctx* ctx);
 
@@ -520,7 +523,13 @@ int32_t thrml_potts_synchronize(thrml_potts* p);
  * them.  Element types are THRML_F32, THRML_BF16, THRML_F16 (indices: THRML_I32, THRML_I64); a pitch is the distance of two
  * rows in elements, at least the row's length; the elements of a row are contiguous.  Pointers are aligned to their element.
  * Inputs and outputs do not overlap except where a call says so.  A call with no rows does nothing.
+ *
+ * Waits inside the product's kernels are bounded.  Where one runs out (a GPU that stands still for seconds), that launch leaves its
+ * output unwritten, in whole or in part, other launches are not touched, and from then on every readout call of the context, and
+ * thrml_ctx_synchronize, return THRML_ERR_TIMEOUT on every thread, until thrml_ctx_reset_waits takes the report down: the caller
+ * first waits for its streams and discards what they held.  Replays of captured graphs report there too.
  * ---------------------------------------------------------------------------------------------- */
+int32_t thrml_ctx_reset_waits(thrml_ctx* ctx);
 #define THRML_F32 0
 #define THRML_BF16 1
 #define THRML_F16 2

@@ -258,6 +258,11 @@ int32_t thrml_ctx_synchronize(thrml_ctx* ctx) {
     CU_TRY(cudaStreamSynchronize(ctx->stream));
     return ctx->check_waits();
 }
+int32_t thrml_ctx_reset_waits(thrml_ctx* ctx) {
+    if (!ctx) return fail(THRML_ERR_INVALID_ARG, "null context");
+    if (ctx->wait_flag) *static_cast<volatile int*>(ctx->wait_flag) = 0;
+    return THRML_OK;
+}
 void* thrml_ctx_stream(thrml_ctx* ctx) { return ctx ? static_cast<void*>(ctx->stream) : nullptr; }
 
 // ---------------------------------------------------------------------------------------------------------

@@ -189,7 +189,7 @@ private:
     cudaError_t status_ = cudaSuccess;
 };
 
-// Body of an entry point: reports a wait that ran out in an earlier call, and turns exceptions into a status.
+// Body of an entry point: refuses while a wait that ran out in an earlier call is reported, and turns exceptions into a status.
 template <class F>
 int32_t guarded(thrml_ctx* ctx, F body) noexcept {
     try {

@@ -224,6 +224,15 @@ __device__ __forceinline__ void quantise_few(const FewTokens& f, int32_t m, int3
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMAs read through the asynchronous proxy
 }
 
+// A wait that runs out: the roles of a CTA tell each other through a word in its shared memory (and the CTAs of a tile each other),
+// which ends their waits and keeps them from writing, and the kernel raises the context's flag as it ends.  Other launches go on.
+__device__ __forceinline__ void tell(dense::SharedWord lost, uint32_t rank, int code) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dense::peer_addr(lost.at, rank)), "r"(code) : "memory");
+}
+__device__ __forceinline__ void report(int* err, int lost) {
+    if (lost) atomicCAS(err, 0, lost);
+}
+
 // A CTA computes a tile of TILE_N channels x BM tokens: the channels are the tensor memory's lanes, so a warp's stores run along
 // a row of the output, and few tokens still fill the MMA's 128 rows.  The CTAs of a cluster (1, 2, 4 or 8) share a tile:
 // each takes a part of K, hands its 32-bit sums over through distributed shared memory, and finishes a part of the tokens.
@@ -242,9 +251,11 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full;
     __shared__ uint32_t tmem_base_slot;
+    __shared__ int lost_word;
     __shared__ uint32_t few_most[FEW ? 16 : 1];
     __shared__ float few_scale[FEW ? 16 : 1];
 
+    const SharedWord lost{smem_u32(&lost_word)};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t split;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(split));
@@ -255,6 +266,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         mbar_init(&acc_full, 1);
+        lost_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -295,7 +307,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
             }
             uint32_t stage = early == STAGES ? 0 : early, phase = early == STAGES ? 1 : 0;
             for (int32_t kt = k_begin + early; kt < k_end; ++kt) {
-                if (!mbar_wait(&empty_bar[stage], phase ^ 1u, g.err, 1)) break;
+                if (!mbar_wait(&empty_bar[stage], phase ^ 1u, lost, 1)) break;
                 mbar_expect_tx(&full_bar[stage], LOAD_BYTES);
                 const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
                 tma_load_2d(dst, &map_w, &full_bar[stage], kt * KB, n0);
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
             uint32_t stage = 0, phase = 0;
             bool alive = true;
             for (int32_t kt = k_begin; kt < k_end; ++kt) {
-                if (!mbar_wait(&full_bar[stage], phase, g.err, 3)) { alive = false; break; }
+                if (!mbar_wait(&full_bar[stage], phase, lost, 3)) { alive = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t w_addr = smem_u32(smem + stage * STAGE_BYTES);
                 const uint64_t dw = make_smem_desc(w_addr), da = make_smem_desc(FEW ? smem_u32(tokens) + (kt - k_begin) * BM * KB : w_addr + W_BYTES);
@@ -334,12 +346,13 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
             }
         };
         if (!FEW) asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' scales
-        const bool alive = mbar_wait(&acc_full, 0, g.err, 4);
+        const bool alive = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, lost, 4));  // the lanes go on together
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
         int32_t* red = reinterpret_cast<int32_t*>(smem + STAGES * STAGE_BYTES);  // [source CTA][token of the share][channel]
         const int32_t share = BM / static_cast<int32_t>(split);
         all_started();
+        if (!alive && lane < static_cast<int>(split)) tell(lost, lane, 4);
         for (int c = (warp - 2) >> 2; c < BM / 16; c += (PROD_THREADS<BM> - 64) / 128) {
             uint32_t acc[16];
             tmem_ld16_issue(taddr + c * 16, acc);
@@ -360,7 +373,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     }
     if (split > 1) {
         cluster_sync_all();  // every CTA's sums have arrived
-        if (warp >= 2) {
+        if (warp >= 2 && !lost.raised()) {
             const int quarter = warp & 3, ch = quarter * 32 + lane;
             const int32_t col = n0 + ch, share = BM / static_cast<int32_t>(split);
             const int32_t* red = reinterpret_cast<const int32_t*>(smem + STAGES * STAGE_BYTES);
@@ -380,6 +393,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (threadIdx.x == 0) report(g.err, lost.value());
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
@@ -424,7 +438,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_base_slot;
+    __shared__ int lost_word;
 
+    const SharedWord lost{smem_u32(&lost_word)};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
@@ -432,6 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        lost_word = 0;
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -466,7 +483,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     phase = early == STAGES ? 1 : 0;
                 }
                 for (int32_t kt = early; kt < g.k_steps; ++kt) {
-                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, g.err, 1)) { alive = false; break; }
+                    if (!mbar_wait(&empty_bar[stage], phase ^ 1u, lost, 1)) { alive = false; break; }
                     if (leader) mbar_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
                     const uint32_t bar = peer_addr(smem_u32(&full_bar[stage]), 0);
                     const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
@@ -483,11 +500,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             bool alive = true;
             for (int32_t tile = first_tile; tile < args.tiles && alive; tile += tile_step, ++it) {
                 const uint32_t buf = it & 1u;
-                if (!mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, g.err, 2)) { alive = false; break; }
+                if (!mbar_wait(&acc_empty[buf], ((it >> 1) & 1u) ^ 1u, lost, 2)) { alive = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t tmem_d = tmem + buf * BM;
                 for (int32_t kt = 0; kt < g.k_steps; ++kt) {
-                    if (!mbar_wait(&full_bar[stage], phase, g.err, 3)) { alive = false; break; }
+                    if (!mbar_wait(&full_bar[stage], phase, lost, 3)) { alive = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t w_addr = smem_u32(smem + stage * STAGE_BYTES);
                     const uint64_t dw = make_smem_desc(w_addr), da = make_smem_desc(w_addr + W_BYTES);
@@ -517,8 +534,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             const uint32_t buf = it & 1u;
             const int32_t col = tn * PAIR_CHANNELS + static_cast<int32_t>(rank) * TILE_N + ch, m0 = tm * BM + half * (BM / 2);
             const float w_scale = col < g.n ? g.w_scale[col] : 0.0f, bias = g.bias && col < g.n ? g.bias[col] : 0.0f;
-            if (!mbar_wait(&acc_full[buf], (it >> 1) & 1u, g.err, 4)) break;
-            __syncwarp();
+            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1u, lost, 4))) break;  // the lanes go on together
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem + buf * BM + half * (BM / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
             T* out = static_cast<T*>(g.out) + static_cast<int64_t>(m0) * g.out_pitch + col;
@@ -544,11 +560,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (lane == 0 && lost.raised()) tell(lost, rank ^ 1, lost.value());
     cluster_sync_all();  // no CTA leaves (or frees tensor memory) while its peer can still reach it
+    if (threadIdx.x == 0) report(g.err, lost.value());
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
+}
+
+// Failure-detection self test: a warp waits as the products do, on a barrier that nothing arrives on, and reports as they do.
+__global__ void k_lose_wait(int* err) {
+    __shared__ uint64_t bar;
+    __shared__ int lost_word;
+    if (threadIdx.x != 0) return;
+    const dense::SharedWord lost{dense::smem_u32(&lost_word)};
+    lost_word = 0;
+    dense::mbar_init(&bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    dense::mbar_wait(&bar, 0, lost, 7);
+    report(err, lost.value());
 }
 
 struct Product {
@@ -750,6 +781,14 @@ int32_t thrml_linear_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int6
         if (done) return THRML_OK;
         if (int32_t rc = run_quant(stream, z)) return rc;
         return run_product(ctx, stream, p);
+    });
+}
+
+int32_t thrml_debug_lose_wait(thrml_ctx* ctx, void* stream) {
+    return guarded(ctx, [&]() -> int32_t {
+        k_lose_wait<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(ctx->wait_flag_dev);
+        CU_TRY(cudaGetLastError());
+        return THRML_OK;
     });
 }
 

@@ -26,7 +26,23 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// Bounded wait on a phase parity.  Returns false (and raises *err) when the limit runs out.
+// Where the roles that wait on each other's barriers tell of a wait that ran out: a word in global memory, or one in the CTA's shared memory.
+struct GlobalWord {
+    int* p;
+    __device__ __forceinline__ bool raised() const { return *reinterpret_cast<volatile int*>(p) != 0; }
+    __device__ __forceinline__ void raise(int code) const { atomicCAS(p, 0, code); }
+};
+struct SharedWord {
+    uint32_t at;
+    __device__ __forceinline__ int value() const {
+        int v;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        return v;
+    }
+    __device__ __forceinline__ bool raised() const { return value() != 0; }
+    __device__ __forceinline__ void raise(int code) const { asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(at), "r"(code) : "memory"); }
+};
+// mbar_wait: bounded wait on a phase parity.  Returns false (and raises the word) when the limit runs out, or another role has raised it.
 // try_wait parks the thread in hardware for up to the hinted time instead of spinning: a polling loop in the producer
 // or MMA warp would take issue slots from the epilogue warps that share its scheduler.  The bound is wall time
 // (about two seconds on the global nanosecond timer), checked between the parked waits.
@@ -36,28 +52,39 @@ __device__ __forceinline__ uint64_t global_ns() {
     return t;
 }
 constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-    const uint32_t addr = smem_u32(bar);
+__device__ __forceinline__ bool mbar_park(uint32_t bar_addr, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar_addr), "r"(parity), "r"(20000u)
+        : "memory");
+    return ok;
+}
+template <class Word>
+__device__ __forceinline__ bool mbar_park_on(uint32_t bar_addr, uint32_t parity, Word word, int code) {
     uint64_t t0 = 0;
     for (uint32_t spin = 0; spin < SPIN_LIMIT; ++spin) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(addr), "r"(parity), "r"(20000u)
-            : "memory");
-        if (ok) return true;
+        if (mbar_park(bar_addr, parity)) return true;
         if ((spin & 15u) == 15u) {
-            if (*reinterpret_cast<volatile int*>(err) != 0) return false;  // another role gave up
+            if (word.raised()) return false;  // another role gave up
             const uint64_t now = global_ns();
             if (t0 == 0) t0 = now;
             else if (now - t0 > WAIT_LIMIT_NS) break;
         }
     }
-    atomicCAS(err, 0, code);
+    word.raise(code);
     return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int code) { return mbar_park_on(smem_u32(bar), parity, GlobalWord{err}, code); }
+// The turns behind the first (20 us) out of line: few waits need any, and inside every wait they cost the small kernels their
+// fetching (one token, 4096 x 4096: 9.6 -> 9.0 us on the GPU) and the large ones issue slots (8192 x 4096 -> 16384: 460 -> 425).
+static __device__ __noinline__ bool mbar_park_longer(uint32_t bar_addr, uint32_t parity, SharedWord word, int code) { return mbar_park_on(bar_addr, parity, word, code); }
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, SharedWord word, int code) {
+    const uint32_t addr = smem_u32(bar);
+    return mbar_park(addr, parity) || mbar_park_longer(addr, parity, word, code);
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y) {

@@ -29,6 +29,10 @@ class Context:
     def synchronize(self):
         check(lib().thrml_ctx_synchronize(self.h))
 
+    def reset_waits(self):
+        """Takes down the report of a readout kernel's wait that ran out; what the context's streams held then is not to be used."""
+        check(lib().thrml_ctx_reset_waits(self.h))
+
     @property
     def stream(self):
         return lib().thrml_ctx_stream(self.h)
