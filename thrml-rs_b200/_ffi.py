@@ -168,11 +168,14 @@ def lib():
         path = _build.OUT
         if not os.path.exists(path):
             raise ImportError(f"{path} is missing: run `python -c 'import __graft_entry__ as g; g.build()'` (needs nvcc); there is no fallback path")
-        _lib = C.CDLL(path)
+        found = C.CDLL(path)
         for name, (res, args) in _SIGNATURES.items():
-            fn = getattr(_lib, name)
+            fn = getattr(found, name, None)
+            if fn is None:
+                raise ImportError(f"{path} has no {name}: it was built from other sources; run `python -c 'import __graft_entry__ as g; g.build()'`")
             fn.restype = res
             fn.argtypes = args
+        _lib = found  # only now: without their types, calls would cut pointers to 32 bits
     return _lib
 
 
