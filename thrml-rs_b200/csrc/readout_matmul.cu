@@ -225,7 +225,8 @@ __device__ __forceinline__ void quantise_few(const FewTokens& f, int32_t m, int3
 }
 
 // A wait that runs out: the roles of a CTA tell each other through a word in its shared memory (and the CTAs of a tile each other),
-// which ends their waits and keeps them from writing, and the kernel raises the context's flag as it ends.  Other launches go on.
+// which ends their waits and keeps them from writing; the kernel then waits, with the same limit, for the loads and MMAs that it has in
+// flight, and raises the context's flag as it ends.  Other launches go on.
 __device__ __forceinline__ void tell(dense::SharedWord lost, uint32_t rank, int code) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dense::peer_addr(lost.at, rank)), "r"(code) : "memory");
 }
@@ -285,6 +286,8 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     };
     // The weights of the first stages do not wait for the tokens to be quantised.
     const int32_t early = min(k_end - k_begin, STAGES);
+    int32_t issued = early;  // loads; whether the MMAs' last commit was made: what is to be settled after a wait that ran out
+    bool committed = false;
     if (threadIdx.x == 0)
         for (int32_t i = 0; i < early; ++i) {
             mbar_expect_tx(&full_bar[i], LOAD_BYTES);
@@ -312,6 +315,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
                 const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
                 tma_load_2d(dst, &map_w, &full_bar[stage], kt * KB, n0);
                 if (!FEW) tma_load_2d(dst + W_BYTES, &map_a, &full_bar[stage], kt * KB, m0);
+                ++issued;
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
@@ -332,6 +336,7 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
             if (alive) umma_commit(&acc_full);
+            committed = alive;
         }
         all_started();
     } else {
@@ -393,7 +398,15 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) report(g.err, lost.value());
+    if (lost.raised()) {
+        if (threadIdx.x == 0) settle_loads(full_bar, STAGES, issued);
+        if (threadIdx.x == 32) {
+            if (!committed) umma_commit(&acc_full);
+            mbar_settle(&acc_full, 0);
+        }
+        if (threadIdx.x == 0) report(g.err, lost.value());
+        __syncwarp();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
@@ -436,9 +449,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], settle_bar;
     __shared__ uint32_t tmem_base_slot;
-    __shared__ int lost_word;
+    __shared__ int lost_word, peer_issued;
 
     const SharedWord lost{smem_u32(&lost_word)};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -449,6 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         lost_word = 0;
+        mbar_init(&settle_bar, 1);
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -460,6 +474,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     cluster_sync_all();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_slot;
+    int32_t issued = 0;  // loads of this CTA
 
     if (warp == 0) {
         if (lane == 0) {
@@ -479,6 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     asm volatile("griddepcontrol.wait;" ::: "memory");
                     for (int32_t i = 0; i < early; ++i)
                         tma_load_2d_pair(smem_u32(smem + i * STAGE_BYTES) + W_BYTES, &map_a, peer_addr(smem_u32(&full_bar[i]), 0), i * KB, m0);
+                    issued = early;
                     stage = early == STAGES ? 0 : early;
                     phase = early == STAGES ? 1 : 0;
                 }
@@ -489,6 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                     const uint32_t dst = smem_u32(smem + stage * STAGE_BYTES);
                     tma_load_2d_pair(dst, &map_w, bar, kt * KB, n0);
                     tma_load_2d_pair(dst + W_BYTES, &map_a, bar, kt * KB, m0);
+                    ++issued;
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -562,7 +579,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (lane == 0 && lost.raised()) tell(lost, rank ^ 1, lost.value());
     cluster_sync_all();  // no CTA leaves (or frees tensor memory) while its peer can still reach it
-    if (threadIdx.x == 0) report(g.err, lost.value());
+    if (lost.raised()) {  // in both CTAs or in none
+        if (threadIdx.x == 0 && !leader)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(smem_u32(&peer_issued), 0)), "r"(issued) : "memory");
+        __syncwarp();
+        cluster_sync_all();
+        if (threadIdx.x == 0 && leader) {  // the barriers of both CTAs' loads are here; of some loads only one has issued its half
+            for (int32_t i = peer_issued; i < issued; ++i) mbar_complete_tx(&full_bar[i % STAGES], STAGE_BYTES);
+            for (int32_t i = issued; i < peer_issued; ++i) mbar_expect_tx(&full_bar[i % STAGES], STAGE_BYTES);
+            settle_loads(full_bar, STAGES, max(issued, peer_issued));
+            report(g.err, lost.value());
+        }
+        if (threadIdx.x == 32 && leader) {
+            umma_commit_pair(smem_u32(&settle_bar));
+            mbar_settle(&settle_bar, 0);
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");

@@ -79,12 +79,27 @@ __device__ __forceinline__ bool mbar_park_on(uint32_t bar_addr, uint32_t parity,
     return false;
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int code) { return mbar_park_on(smem_u32(bar), parity, GlobalWord{err}, code); }
-// The turns behind the first (20 us) out of line: few waits need any, and inside every wait they cost the small kernels their
-// fetching (one token, 4096 x 4096: 9.6 -> 9.0 us on the GPU) and the large ones issue slots (8192 x 4096 -> 16384: 460 -> 425).
+// The turns behind the first (20 us) out of line: few waits need any, and inside every wait they cost issue slots
+// (8192 x 4096 -> 16384: 460 -> 425 us).
 static __device__ __noinline__ bool mbar_park_longer(uint32_t bar_addr, uint32_t parity, SharedWord word, int code) { return mbar_park_on(bar_addr, parity, word, code); }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, SharedWord word, int code) {
     const uint32_t addr = smem_u32(bar);
     return mbar_park(addr, parity) || mbar_park_longer(addr, parity, word, code);
+}
+
+// For what a kernel has in flight when its roles have given up: nobody to tell, and the same limit.
+struct NoWord {
+    __device__ __forceinline__ bool raised() const { return false; }
+    __device__ __forceinline__ void raise(int) const {}
+};
+static __device__ __noinline__ void mbar_settle(uint64_t* bar, uint32_t parity) { mbar_park_on(smem_u32(bar), parity, NoWord{}, 0); }
+// The last of `issued` loads in turn on a ring of barriers: those that no later one has waited for.
+static __device__ __noinline__ void settle_loads(uint64_t* ring, int32_t stages, int32_t issued) {
+    for (int32_t i = max(issued - stages, 0); i < issued; ++i) mbar_settle(ring + i % stages, i / stages & 1);
+}
+// Bytes that will not come count as come.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x, int32_t y) {
