@@ -98,3 +98,24 @@ def test_two_threads_of_a_context(T):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("m, k, n", [(3, 100, 300), (20, 1000, 777), (64, 512, 5000), (700, 640, 9000)])  # one or two launches, K split, pairs
+def test_one_workspace_for_call_behind_call(T, m, k, n):
+    """The product takes the scales that the quantiser of its own call wrote, though both are at work at once and all calls share their workspace."""
+    g = torch.Generator("cuda").manual_seed(m)
+    w, ws = T.quantize_rows(torch.randn(n, k, generator=g, device="cuda"))
+    xs = [torch.randn(m, k, generator=g, device="cuda") * 10.0**i for i in range(-6, 6)]
+    want = [T.int8_matmul(*T.quantize_rows(x), w, ws) for x in xs]
+    pitch = (k + 15) // 16 * 16
+    q, scale = torch.empty(m, pitch, dtype=torch.int8, device="cuda"), torch.empty(m, device="cuda")
+    outs = [torch.empty(m, n, device="cuda") for _ in xs]
+    h, stream = T.default_context(0).h, torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x, out in zip(xs, outs):
+            T._ffi.check(T.lib().thrml_linear_i8(h, stream, m, n, k, x.data_ptr(), 0, k, q.data_ptr(), pitch, scale.data_ptr(), w.data_ptr(), w.stride(0), ws.data_ptr(), None, out.data_ptr(), 0, n))
+        torch.cuda.synchronize()
+        for out, v in zip(outs, want):
+            assert torch.equal(out, v)
+            out.zero_()

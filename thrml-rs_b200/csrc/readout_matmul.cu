@@ -297,9 +297,10 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
     uint8_t* tokens = smem + STAGES * STAGE_BYTES + (split > 1 ? sizeof(int32_t) * TILE_N * BM : 0);  // FEW: a tile of BM x KB per step
     if constexpr (FEW) quantise_few<X>(few, g.m, k_begin * KB, min(k_end * KB, few.k), tokens, few_scale, few_most, PROD_THREADS<BM>);
     if (FEW) __syncthreads();
+    // By plain loads: the kernel that writes the scales may be at work when this one starts.
     auto a_scale = [&](int32_t token) {
         if constexpr (FEW) return few_scale[token];
-        else return __ldg(g.a_scale + token);
+        else return g.a_scale[token];
     };
 
     if (warp == 0) {
@@ -344,12 +345,6 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
         const int32_t col = n0 + ch;
         const float w_scale = col < g.n ? g.w_scale[col] : 0.0f, bias = g.bias && col < g.n ? g.bias[col] : 0.0f;
         T* out = static_cast<T*>(g.out) + col;
-        auto finish = [&](int32_t token, int32_t acc) {
-            if (token < g.m && col < g.n) {
-                const float y = __int2float_rn(acc) * a_scale(token) * w_scale;
-                out[token * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
-            }
-        };
         if (!FEW) asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' scales
         const bool alive = __all_sync(0xffffffffu, mbar_wait(&acc_full, 0, lost, 4));  // the lanes go on together
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -363,9 +358,18 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
             tmem_ld16_issue(taddr + c * 16, acc);
             tmem_ld_wait();
             if (split == 1) {
-                if (alive)
+                const int32_t first = m0 + c * 16, left = g.m - first;  // tokens from here on
+                if (alive && col < g.n) {
+                    float scales[16];  // loaded before the stores, which hold later loads back
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) finish(m0 + c * 16 + j, static_cast<int32_t>(acc[j]));
+                    for (int j = 0; j < 16; ++j) scales[j] = j < left ? a_scale(first + j) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (j < left) {
+                            const float y = __int2float_rn(static_cast<int32_t>(acc[j])) * scales[j] * w_scale;
+                            out[(first + j) * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
+                        }
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
@@ -561,13 +565,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
                 tmem_ld16_issue(taddr + c * 16, acc);
                 tmem_ld_wait();
                 const int32_t left = g.m - (m0 + c * 16);  // tokens from here on
-                if (col < g.n)
+                if (col < g.n) {
+                    float scales[16];  // by plain loads (see k_product), before the stores
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) scales[j] = j < left ? g.a_scale[m0 + c * 16 + j] : 0.0f;
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (j < left) {
-                            const float y = __int2float_rn(static_cast<int32_t>(acc[j])) * __ldg(g.a_scale + m0 + c * 16 + j) * w_scale;
+                            const float y = __int2float_rn(static_cast<int32_t>(acc[j])) * scales[j] * w_scale;
                             out[(c * 16 + j) * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
                         }
+                }
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
