@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <new>
 #include <string>
@@ -207,13 +208,13 @@ int32_t guarded(thrml_ctx* ctx, F body) noexcept {
     }
 }
 
-// Lets a kernel have more than 48 KB of dynamic shared memory, once for each device.
+// Lets a kernel have more than 48 KB of dynamic shared memory, once for each device (threads that come at once do it twice).
 template <auto KERNEL>
 int32_t allow_shared(const thrml_ctx* ctx, size_t bytes) {
-    static bool done[64] = {};
-    if (ctx->device < 64 && done[ctx->device]) return THRML_OK;
+    static std::atomic<bool> done[64];
+    if (ctx->device < 64 && done[ctx->device].load(std::memory_order_acquire)) return THRML_OK;
     CU_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
-    if (ctx->device < 64) done[ctx->device] = true;
+    if (ctx->device < 64) done[ctx->device].store(true, std::memory_order_release);
     return THRML_OK;
 }
 
