@@ -5,6 +5,7 @@ written on top of them.
 """
 import ctypes as C
 import os
+import threading
 
 import numpy as np
 
@@ -16,6 +17,7 @@ SAMPLER_CATEGORICAL = 1
 SAMPLER_SOFTMAX = 2
 
 _default_ctx = {}
+_default_lock = threading.Lock()
 
 
 class Context:
@@ -53,9 +55,10 @@ def default_context(device_id=None):
     """Process-wide context; one process drives one GPU (LOCAL_RANK selects it under torchrun)."""
     if device_id is None:
         device_id = int(os.environ.get("LOCAL_RANK", "0"))
-    if device_id not in _default_ctx:
-        _default_ctx[device_id] = Context(device_id)
-    return _default_ctx[device_id]
+    with _default_lock:  # of two contexts made at once, one would be destroyed under the thread that made it
+        if device_id not in _default_ctx:
+            _default_ctx[device_id] = Context(device_id)
+        return _default_ctx[device_id]
 
 
 class Comm:
