@@ -58,3 +58,24 @@ print("all the same")
 def test_first_readout_calls_from_eight_threads():
     done = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "all the same" in done.stdout, done.stderr[-2000:]
+
+
+CLOSED = """
+import torch
+import __graft_entry__ as graft
+T = graft.load_package()
+x = torch.ones(2, 32, device="cuda")
+T.quantize_rows(x)
+torch.cuda.synchronize()
+T.default_context(0).close()
+try:
+    T.quantize_rows(x)
+except T.ThrmlError as e:
+    print("refused", e)
+"""
+
+
+@pytest.mark.gpu
+def test_a_closed_context_is_refused():
+    done = subprocess.run([sys.executable, "-c", CLOSED], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "refused" in done.stdout and "null context" in done.stdout, done.stderr[-2000:]

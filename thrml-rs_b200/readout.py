@@ -17,7 +17,7 @@ torch = None  # imported by the first call: the rest of the package works on hos
 _TYPES = {}
 _FLOATS, _WHOLE = (0, 1, 2), (3, 4)
 _raw_stream = None
-_handles = {}  # device index -> the context's handle
+_contexts = {}  # device index -> its context
 
 
 def _refuse(why):
@@ -41,13 +41,13 @@ def _device(x, name):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         _refuse(f"{name} has to be a CUDA tensor")
     index = x.get_device()
-    h = _handles.get(index)
-    if h is None:
+    ctx = _contexts.get(index)
+    if ctx is None:
         if index not in _eng._default_ctx and torch.cuda.is_current_stream_capturing():
             _refuse("the first call on a device makes its context, which a stream capture cannot hold: make one call before the capture")
         with torch.cuda.device(index):  # making a context changes the current device
-            h = _handles[index] = _eng.default_context(index).h
-    return h, _raw_stream(index), index
+            ctx = _contexts[index] = _eng.default_context(index)
+    return ctx.h, _raw_stream(index), index  # of a context that was closed None, which every call refuses
 
 
 def _rows(x, name, index, kinds=_FLOATS, rows=None, cols=None):
