@@ -161,3 +161,24 @@ def test_draw_categories_large_beta(T, dtype, beta, r, v):
     assert torch.equal(T.draw_categories(x, 77, beta=b).cpu(), draw64(x, uniforms(r, v, 77), b))
     noise = torch.rand(r, v, generator=gen(9), device="cuda").clamp_(1e-6, 0.999999)
     assert torch.equal(T.draw_categories(x, 77, beta=b, noise=noise).cpu(), draw64(x, noise.cpu().numpy(), b))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_outputs_beside_inputs_and_over_them(T, dtype):
+    """Columns of one buffer may hold input and output side by side; an output that shares elements with an input is refused."""
+    both = torch.randn(6, 2048, generator=gen(4), device="cuda").to(dtype)
+    x, y = both[:, :1024], both[:, 1024:]
+    w, ws = T.quantize_rows(torch.randn(1024, 1024, generator=gen(5), device="cuda"))
+    ids, teacher = torch.arange(4, device="cuda")[None].repeat(6, 1), torch.zeros(6, 4, device="cuda")
+    beta = torch.ones(6, device="cuda")
+    mask = torch.full((6, 32), 0x55555555, dtype=torch.int32, device="cuda")
+    for f in (lambda o: T.int8_linear(x, w, ws, out=o), lambda o: T.adjust_logits(x, mask=mask, out=o), lambda o: T.distill_step(x, ids, teacher, out=o)[1],
+              lambda o: T.distill_grad(x, beta, ids, teacher, out=o)):
+        want = f(None)
+        assert f(y) is y and torch.equal(y, want)
+        for o in (both[:, 1:1025], both[:, 1023:2047], both.view(-1)[8:8 + 6 * 1024].view(6, 1024)):
+            with pytest.raises(T.ThrmlError, match="overlap"):
+                f(o)
+    for f in (lambda: T.int8_linear(x, w, ws, out=x), lambda: T.distill_step(x, ids, teacher, out=x), lambda: T.distill_grad(x, beta, ids, teacher, out=x)):
+        with pytest.raises(T.ThrmlError):
+            f()

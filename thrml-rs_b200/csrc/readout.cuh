@@ -169,6 +169,26 @@ inline bool is_index_type(int32_t t) { return t == THRML_I32 || t == THRML_I64; 
 inline size_t type_size(int32_t t) { return t == THRML_F32 || t == THRML_I32 ? 4 : t == THRML_I64 ? 8 : 2; }
 inline bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Rows of `width` elements `pitch` apart, by their bytes.
+struct Area {
+    uintptr_t at;
+    int64_t rows, width, pitch;
+    Area(const void* p, size_t size, int64_t r, int64_t w, int64_t pitch_) : at(reinterpret_cast<uintptr_t>(p)), rows(r), width(w * static_cast<int64_t>(size)), pitch(pitch_ * static_cast<int64_t>(size)) {}
+};
+// Whether two areas share bytes (rows of one pitch may lie beside each other in one buffer; of two pitches, they are taken to share).
+inline bool overlap(const Area& a, const Area& b) {
+    using Wide = __int128;
+    if (!a.at || !b.at || a.rows < 1 || b.rows < 1 || a.width < 1 || b.width < 1) return false;
+    const Wide a_end = static_cast<Wide>(a.at) + static_cast<Wide>(a.rows - 1) * a.pitch + a.width, b_end = static_cast<Wide>(b.at) + static_cast<Wide>(b.rows - 1) * b.pitch + b.width;
+    if (a.at >= b_end || b.at >= a_end) return false;
+    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+    const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+    if ((a.rows == 1 && b.rows == 1) || pitch < 1) return true;
+    const Wide apart = static_cast<Wide>(b.at) - static_cast<Wide>(a.at);
+    const Wide behind = ((apart % pitch) + pitch) % pitch;  // of b's rows behind a's
+    return behind < a.width || behind + b.width > pitch;
+}
+
 // The context's device for the length of a call; the caller's current device comes back.
 class OnDevice {
 public:

@@ -942,6 +942,7 @@ int32_t distill(thrml_ctx* ctx, void* stream, int mode, int64_t rows, int32_t ty
     if (mode != LOSS) {
         if (int32_t rc = check_rows("grad", rows, g.cols, g.grad, type, g.grad_pitch)) return rc;
         if (rows && g.grad == g.logits) return fail(THRML_ERR_INVALID_ARG, "grad must not be the logits themselves");
+        if (overlap(Area(g.grad, type_size(type), rows, g.cols, g.grad_pitch), Area(g.logits, type_size(type), rows, g.cols, g.pitch))) return fail(THRML_ERR_INVALID_ARG, "grad overlaps the logits");
     }
     if (g.top < 0 || g.top > TOP_MAX) return fail(THRML_ERR_INVALID_ARG, "top is not within 0 and 1024");
     if (!is_index_type(g.ids_type)) return fail(THRML_ERR_INVALID_ARG, "ids: the element type is not an index type");
@@ -1002,6 +1003,8 @@ int32_t thrml_adjust_logits(thrml_ctx* ctx, void* stream, int64_t rows, int64_t 
             while (2 * per_row <= most && rows * per_row < 2 * ctx->sm_count && span / (2 * per_row) >= 256) per_row *= 2;
             const int64_t share = ((span + per_row - 1) / per_row + 63) / 64 * 64;
             if (rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
+            if (out != logits && overlap(Area(out, sizeof(T), rows, cols, out_pitch), Area(logits, sizeof(T), rows, cols, pitch)))
+                return fail(THRML_ERR_INVALID_ARG, "out overlaps the logits without being them");
             // half of a full share's positions at a time (long histories) take 4 bytes each, the whole share 2
             const int64_t count_bytes = std::max<int64_t>(2 * share, 4 * std::min<int64_t>(share, ADJUST_SHARE<T> / 2));
             const AdjustArgs g{logits, out, pitch, out_pitch, static_cast<int32_t>(cols), static_cast<int32_t>(share), static_cast<int32_t>(per_row), static_cast<int32_t>(count_bytes / 4), *rules};

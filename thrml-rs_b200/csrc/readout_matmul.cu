@@ -658,6 +658,14 @@ int32_t check_product(const Product& p) {
     return check_matrix8("w", p.w, p.k, p.w_pitch);
 }
 
+int32_t check_apart(const Product& p) {
+    const Area out(p.out, type_size(p.out_type), p.m, p.n, p.out_pitch);
+    if (overlap(out, Area(p.a, 1, p.m, p.k, p.a_pitch)) || overlap(out, Area(p.w, 1, p.n, p.k, p.w_pitch)) || overlap(out, Area(p.a_scale, 4, 1, p.m, p.m)) ||
+        overlap(out, Area(p.w_scale, 4, 1, p.n, p.n)) || overlap(out, Area(p.bias, 4, 1, p.n, p.n)))
+        return fail(THRML_ERR_INVALID_ARG, "out overlaps an input");
+    return THRML_OK;
+}
+
 template <int BM, class T, class X>
 int32_t launch_product(thrml_ctx* ctx, cudaStream_t stream, const Product& p, int split, const FewTokens& few) {
     CUtensorMap map_w, map_a;
@@ -804,6 +812,7 @@ int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int6
     return guarded(ctx, [&]() -> int32_t {
         const Product p{m, n, k, a, a_pitch, a_scale, w, w_pitch, w_scale, bias, out, out_type, out_pitch, false};
         if (int32_t rc = check_product(p)) return rc;
+        if (int32_t rc = check_apart(p)) return rc;
         return run_product(ctx, stream, p);
     });
 }
@@ -815,7 +824,10 @@ int32_t thrml_linear_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int6
         if (int32_t rc = check_product(p)) return rc;
         const Quant z{m, k, x, x_type, x_pitch, q, q_pitch, scale};
         if (int32_t rc = check_quant(z)) return rc;
+        if (int32_t rc = check_apart(p)) return rc;
         if (m == 0 || n == 0) return THRML_OK;
+        // CTAs that quantise the tokens themselves read x while others write
+        if (overlap(Area(out, type_size(out_type), m, n, out_pitch), Area(x, type_size(x_type), m, k, x_pitch))) return fail(THRML_ERR_INVALID_ARG, "out overlaps x");
         bool done = false;
         Product alone = p;
         alone.after_quantising = false;

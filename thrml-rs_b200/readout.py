@@ -4,7 +4,7 @@ thrml_draw_categories, thrml_distill_* of include/thrml_b200.h).
 
 A row is one sequence or chain.  Every call runs on the tensors' own device and on that device's current torch stream,
 returns before the GPU is done, and can be captured into a CUDA graph once a call has been made on the device before.
-Arguments that do not fit raise ThrmlError.  Gradients are returned, as by `estimate_kl_grad`; nothing here is recorded by
+Arguments that do not fit raise ThrmlError, an `out` that shares memory with an input among them (`adjust_logits` alone may work in place).  Gradients are returned, as by `estimate_kl_grad`; nothing here is recorded by
 autograd.
 """
 import ctypes as C
