@@ -182,3 +182,9 @@ def test_outputs_beside_inputs_and_over_them(T, dtype):
     for f in (lambda: T.int8_linear(x, w, ws, out=x), lambda: T.distill_step(x, ids, teacher, out=x), lambda: T.distill_grad(x, beta, ids, teacher, out=x)):
         with pytest.raises(T.ThrmlError):
             f()
+
+
+@pytest.mark.parametrize("offset", [-1, (1 << 32) - 3, 1 << 63, 1 << 64, (1 << 64) + 5, -(1 << 64)])
+def test_draw_categories_refuses_offsets_of_any_size(T, offset):
+    with pytest.raises(T.ThrmlError, match="row_offset"):
+        T.draw_categories(torch.zeros(4, 64, device="cuda"), 1, row_offset=offset)

@@ -257,6 +257,8 @@ def draw_categories(logits, key, *, beta=None, row_offset=0, noise=None, out=Non
     key = key.seed() if hasattr(key, "seed") else int(key)
     if not 0 <= key < 1 << 64:
         _refuse("key is not a 64-bit number")
+    if not 0 <= row_offset <= (1 << 32) - rows:  # here too: what does not fit 64 bits would be cut on its way
+        _refuse("row_offset is out of range")
     _check(lib().thrml_draw_categories(h, stream, rows, cols, logits.data_ptr(), kind, pitch, _vector(beta, "beta", index, torch.float32, rows), key, int(row_offset), u, u_pitch,
                                        out.data_ptr()))
     return out
