@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_readout import E, IDS, TINY, TYPES, draw64, gen, half, near, uniforms  # noqa: F401
+from test_gpu_readout import adjust64, E, IDS, TINY, TYPES, draw64, gen, half, near, uniforms  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +188,18 @@ def test_outputs_beside_inputs_and_over_them(T, dtype):
 def test_draw_categories_refuses_offsets_of_any_size(T, offset):
     with pytest.raises(T.ThrmlError, match="row_offset"):
         T.draw_categories(torch.zeros(4, 64, device="cuda"), 1, row_offset=offset)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_adjust_logits_any_repetition(T, dtype):
+    """Penalties from the smallest to the largest: the reciprocal of many of them is no f32, their quotients are."""
+    reps = torch.tensor([2.0**-149, 2.0**-140, 1e-39, 2.0**-126, 1e-3, 1.0, 7.0, 1e30, 1e38, 3e38], device="cuda")
+    n = 64
+    x = torch.logspace(-40, 38, n, device="cuda")[None].repeat(10, 1)
+    x[:, ::3] *= -1
+    x = x.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype)
+    rules = dict(history=torch.arange(n, device="cuda").repeat(10), history_ptr=torch.arange(11, device="cuda") * n, repetition=reps)
+    got = T.adjust_logits(x, **rules)
+    want, _ = adjust64(x, rules)
+    want = want.float().to(dtype).double()  # one rounding to f32 and one to the type: beyond their range an infinity
+    near(got, want, (2 * E + 2 * half(dtype)) * want.abs().nan_to_num(0, 0, 0) + TINY[dtype])

@@ -43,7 +43,7 @@ __device__ __forceinline__ uint4 nothing_16() {
 //
 // Every logit is read and written once.  A CTA copies a share of a row into shared memory, ADJUST_PIECES 16-byte pieces a thread,
 // in flight together; meanwhile it counts there those of the row's tokens that fall into the share (integer atomics, so the counts
-// do not depend on their order).  A count has 16 bits, and 32 in rows of 2^15 tokens or more, which are done half a share at a time.
+// do not depend on their order).  A count has 16 bits, and 32 in rows of 2^15 tokens or more (and where the repetition penalty has no reciprocal in f32), which are done half a share at a time.
 // Every CTA of a row reads the whole history, from L2 after the first.  256 x 131072 bf16 with 4096 tokens, biases and masks 56 us =
 // 2.4 TB/s, bound by instruction issue; without any rule 23, by memory.
 // Categories with a bias are finished by a thread of their own, before the pass over the share, which leaves out what a bitmap
@@ -84,8 +84,13 @@ __device__ __forceinline__ uint4 close_16(const uint4& raw, uint32_t open) {
 // What the penalties make of a logit that was seen, `told` times behind the prompt.
 struct Penalties {
     float repetition, per_repetition, frequency, presence;
-    __device__ __forceinline__ float operator()(float x, uint32_t told) const {
-        x *= x > 0.0f ? per_repetition : repetition;
+    // One division a row instead of one a category (1.5 steps of f32 at most; 256 x 131072 bf16 56 us, with divisions 60), where the
+    // reciprocal is a normal number.
+    __device__ __forceinline__ bool has_reciprocal() const { return repetition >= 0x1p-126f && repetition <= 0x1p126f; }
+    template <bool DIVIDE>
+    __device__ __forceinline__ float of(float x, uint32_t told) const {
+        if (DIVIDE) x = x > 0.0f ? __fdiv_rn(x, repetition) : x * repetition;
+        else x *= x > 0.0f ? per_repetition : repetition;
         return told ? x - fmaf(frequency, static_cast<float>(told), presence) : x;
     }
 };
@@ -152,8 +157,7 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
     const int32_t* ids = ru.bias_ids + b0;
     const int64_t split = has_history && ru.n_prompt ? min(h1, h0 + max(ru.n_prompt[row], 0)) : h0;
     const float repetition = ru.repetition ? ru.repetition[row] : 1.0f;
-    const Penalties penalise{repetition, __fdiv_rn(1.0f, repetition),  // one division a row instead of one a category: 1.5 steps of f32 at most
-                             ru.frequency ? ru.frequency[row] : 0.0f, ru.presence ? ru.presence[row] : 0.0f};
+    const Penalties penalties{repetition, __fdiv_rn(1.0f, repetition), ru.frequency ? ru.frequency[row] : 0.0f, ru.presence ? ru.presence[row] : 0.0f};
     const int64_t m = !ru.mask ? -1 : ru.mask_rows ? ru.mask_rows[row] : row;
     const uint32_t* mask = ru.mask && m >= 0 && m < ru.n_masks ? ru.mask + m * ru.mask_pitch : nullptr;
     const bool wide = pieces.same_phase(out);
@@ -177,6 +181,7 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
     // Pieces s0 .. s1 of each thread, the positions [begin, stop), with counts of BITS bits.
     auto pass = [&](auto bits, int s0, int s1, int32_t begin, int32_t stop) {
         constexpr int BITS = decltype(bits)::value;
+        auto penalise = [&](float x, uint32_t told) { return penalties.of<BITS == 32>(x, told); };
         const Counts<BITS> count{reinterpret_cast<uint32_t*>(counts)};
         if (has_history) {
             if (s0 > 0)  // the second half's; the first begin at 0
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
             pieces.store(out, at, bits, wide, done);
         }
     };
-    if (h1 - h0 < 1 << 15) {
+    if (h1 - h0 < 1 << 15 && penalties.has_reciprocal()) {
         pass(Count<16>{}, 0, ADJUST_PIECES, from, to);
     } else {
         const int32_t half = from + ADJUST_PIECES / 2 * ADJUST_THREADS * V;
