@@ -203,3 +203,41 @@ def test_adjust_logits_any_repetition(T, dtype):
     want, _ = adjust64(x, rules)
     want = want.float().to(dtype).double()  # one rounding to f32 and one to the type: beyond their range an infinity
     near(got, want, (2 * E + 2 * half(dtype)) * want.abs().nan_to_num(0, 0, 0) + TINY[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("n, times, top", [(3001, 90, 70), (9001, 100, 129), (140003, 20, 40)])
+def test_distill_large_logits_with_lists(T, dtype, n, times, top):
+    """Lists of a warp, of four, and rows of several CTAs, whose sums a gradient forms again."""
+    g = gen(top)
+    for size in (300.0, 1e4, 1e9, 1e30):
+        if size > torch.finfo(dtype).max:
+            continue
+        x = large_rows(size, n, dtype, n)
+        ids = torch.randint(-1, n + 1, (5, top), generator=g, device="cuda")
+        ids[2] = torch.tensor([n // 2, n - 1], device="cuda").repeat(top)[:top]
+        check_large(T, x, ids, torch.randn(5, top, generator=g, device="cuda"), 0.7, times)
+
+
+@pytest.mark.parametrize("dtype, n, rows", [(torch.float32, 1048601, 1), (torch.float32, 1048601, 40), (torch.bfloat16, 4500001, 2), (torch.float16, 2097200, 38)])
+def test_distill_rows_beyond_4_mb(T, dtype, n, rows):
+    """A gradient's CTAs share such rows' sums, where they form them again: ordinary rows, a large one among them, one of the lowest value."""
+    x = torch.randn(rows, n, generator=gen(6), device="cuda") * 3
+    x[-1] = torch.finfo(dtype).min
+    if rows > 1:
+        x[0] += 1000
+    x = x.to(dtype)
+    ids = torch.randint(0, n, (rows, 6), generator=gen(7), device="cuda")
+    ids[:, 3] = n - 1
+    teacher = torch.randn(rows, 6, generator=gen(8), device="cuda")
+    loss, lse = T.distill_loss(x, ids, teacher, beta=0.5)
+    grad = T.distill_grad(x, lse, ids, teacher, beta=0.5)
+    loss2, grad2 = T.distill_step(x, ids, teacher, beta=0.5)
+    for i in {0, rows // 2, rows - 1}:
+        one = slice(i, i + 1)
+        L, S, G, el, es, eg, given = distill64(x[one], ids[one], teacher[one], 0.5)
+        near(lse[one], S, es)
+        near(loss[one], L, el)
+        near(loss2[one], L, el)
+        for got, more in ((grad2, 0.0), (grad, given)):
+            near(got[one], G, eg + more + half(dtype) * (G.abs() + eg + more) + TINY[dtype])

@@ -505,6 +505,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 4) k_draw(const __grid_constant_
 constexpr int SOFTMAX_THREADS = 256;
 constexpr int64_t SOFTMAX_BYTES = 64 << 10;  // of a row per CTA
 constexpr int LIST_WARPS = 4;
+constexpr int SUMMED_APART = 64;  // 4 MB of a row
 enum Distill { LOSS, GRAD, STEP };
 
 struct DistillArgs {
@@ -518,8 +519,9 @@ struct DistillArgs {
     void* grad;
     int64_t rows, pitch, ids_pitch, teacher_pitch, grad_pitch;
     int32_t cols, top, ids_type, teacher_type;
-    float beta;
+    float beta, per_beta;
     int32_t share, per_row;  // positions of a row per CTA, CTAs per row
+    bool joined;
 };
 
 // beta's range: a finite difference of two logits that f32 cannot hold is then weight 0, and base 2 does not overflow.
@@ -630,17 +632,42 @@ __device__ __forceinline__ Partial sum_of(const Share<T>& s, float b2, int tid) 
     if (!(sum < 0x1p100f)) return sum_carefully<T, THREADS>(s, b2, tid);  // an infinite reference among them
     return Partial{ref, sum};
 }
-// The sum of a whole row, by a CTA of THREADS threads or a warp (rows whose lse a gradient does not take as it is).
+// A share's sum by a CTA of THREADS threads (or a warp), of whose warps it joins the parts.
 template <class T, int THREADS>
-__device__ __noinline__ Partial sum_again(const T* logits, int32_t cols, float b2, int tid, Partial* warps) {
-    Partial p = sum_of<T, THREADS>(Share<T>(logits, cols, 0, cols + VEC<T>), b2, tid);
+__device__ __forceinline__ Partial sum_of_cta(const Share<T>& s, float b2, int tid, Partial* warps) {
+    Partial p = sum_of<T, THREADS>(s, b2, tid);
     if (THREADS > 32) {
         if ((tid & 31) == 0) warps[tid >> 5] = p;
         __syncthreads();
-        p = warps[0];
-        for (int w = 1; w < THREADS / 32; ++w) p.join(warps[w], b2);
+        p = warps[tid & (THREADS / 32 - 1)];
+        for (int d = THREADS / 64; d; d >>= 1) p.join(Partial{__shfl_xor_sync(0xffffffffu, p.ref, d), __shfl_xor_sync(0xffffffffu, p.sum, d)}, b2);
+        p = Partial{__shfl_sync(0xffffffffu, p.ref, 0), __shfl_sync(0xffffffffu, p.sum, 0)};
     }
     return p;
+}
+// The sum of a row from those of its cluster's CTAs, which have all arrived once at the cluster's barrier.
+__device__ __forceinline__ Partial sum_of_cluster(Partial p, float b2, int tid, int32_t part, int32_t per_row, Partial* ctas) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row has started
+    if (tid < per_row) {
+        const uint32_t to = dense::peer_addr(dense::smem_u32(&ctas[part]), tid);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(p.ref), "f"(p.sum) : "memory");
+    }
+    dense::cluster_sync_all();
+    p = ctas[0];
+    for (int c = 1; c < per_row; ++c) p.join(ctas[c], b2);
+    return p;
+}
+// The sums of a row whose lse a gradient does not take as it is, out of line: by the CTA (or warp) alone, which reads all of the row.
+template <class T, int THREADS>
+__device__ __noinline__ Partial sum_again(const T* logits, int32_t cols, float b2, int tid, Partial* warps) {
+    return sum_of_cta<T, THREADS>(Share<T>(logits, cols, 0, cols + VEC<T>), b2, tid, warps);
+}
+// And by the row's cluster, of which the CTA reads its share.
+template <class T>
+__device__ __noinline__ Partial sum_again_together(const T* logits, int32_t cols, int32_t share, float b2, int tid, int32_t part, int32_t per_row, Partial* warps, Partial* ctas) {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const Partial p = sum_of_cta<T, SOFTMAX_THREADS>(Share<T>(logits, cols, part * share, share), b2, tid, warps);
+    return sum_of_cluster(p, b2, tid, part, per_row, ctas);
 }
 
 // q of a row, from the joined parts of its sum or from its lse: 2^(b2 (l - ref) - sum2).
@@ -649,10 +676,10 @@ struct Softmax {
     bool empty;
     __device__ __forceinline__ static Softmax of(Partial p) { return of(p.ref, p.sum == INFINITY || (p.ref == -INFINITY && p.sum != 0.0f) ? NAN : log2f(p.sum)); }
     __device__ __forceinline__ static Softmax of(float ref, float sum2) { return Softmax{ref, sum2, ref == -INFINITY && sum2 == -INFINITY}; }
-    // lse as beta ref + a rest, so that here too the difference comes first.
-    __device__ __forceinline__ static Softmax of_lse(float lse, float beta) {
-        const float ref = lse / beta;
-        return Softmax{ref, LOG2E * static_cast<float>(lse - static_cast<double>(beta) * ref), false};
+    // lse as beta ref + a rest (ref is near lse / beta, whatever per_beta's rounding), so that here too the difference comes first.
+    __device__ __forceinline__ static Softmax of_lse(float lse, float beta, float per_beta) {
+        const float ref = lse * per_beta;
+        return Softmax{ref, LOG2E * fmaf(-beta, ref, lse), false};
     }
     // What is taken from a logit, and from the exponent: a row with nothing has q = 0.
     __device__ __forceinline__ float back() const { return empty ? 0.0f : ref; }
@@ -778,9 +805,9 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
     const int tid = threadIdx.x, lane = tid & 31;
     const int64_t row = g.per_row == 1 ? blockIdx.x : blockIdx.x / g.per_row;
     const int32_t part = static_cast<int32_t>(blockIdx.x - row * g.per_row);
-    const bool joined = MODE != GRAD && g.per_row > 1;  // the CTAs of a row form a cluster
+    const bool joined = g.joined;  // the CTAs of a row form a cluster
     if (!WHOLE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (joined) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    if (MODE != GRAD && joined) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const float weight = g.weight ? g.weight[row] : 1.0f;  // 0: padding, nothing of the row is read
     const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
     const Share<T> s(logits, g.cols, part * g.share, g.share);
@@ -789,26 +816,14 @@ __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_con
     if (MODE == GRAD) {
         if (weight != 0.0f) {
             const float lse = g.lse_in[row];
-            soft = fabsf(lse) > LSE_KEPT ? Softmax::of(sum_again<T, SOFTMAX_THREADS>(logits, g.cols, b2, tid, warps)) : Softmax::of_lse(lse, g.beta);
+            if (!(fabsf(lse) > LSE_KEPT)) soft = Softmax::of_lse(lse, g.beta, g.per_beta);
+            else if (joined) soft = Softmax::of(sum_again_together<T>(logits, g.cols, g.share, b2, tid, part, g.per_row, warps, ctas));
+            else soft = Softmax::of(sum_again<T, SOFTMAX_THREADS>(logits, g.cols, b2, tid, warps));
         }
     } else {
         Partial p{-INFINITY, 0.0f};
-        if (weight != 0.0f) p = sum_of<T, SOFTMAX_THREADS>(s, b2, tid);
-        if (lane == 0) warps[tid >> 5] = p;
-        __syncthreads();
-        p = warps[lane & (SOFTMAX_THREADS / 32 - 1)];
-        for (int d = SOFTMAX_THREADS / 64; d; d >>= 1) p.join(Partial{__shfl_xor_sync(0xffffffffu, p.ref, d), __shfl_xor_sync(0xffffffffu, p.sum, d)}, b2);
-        p = Partial{__shfl_sync(0xffffffffu, p.ref, 0), __shfl_sync(0xffffffffu, p.sum, 0)};
-        if (joined) {
-            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA of the row has started
-            if (tid < g.per_row) {
-                const uint32_t to = dense::peer_addr(dense::smem_u32(&ctas[part]), tid);
-                asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(p.ref), "f"(p.sum) : "memory");
-            }
-            dense::cluster_sync_all();
-            p = ctas[0];
-            for (int c = 1; c < g.per_row; ++c) p.join(ctas[c], b2);
-        }
+        if (weight != 0.0f) p = sum_of_cta<T, SOFTMAX_THREADS>(s, b2, tid, warps);  // weight is the row's
+        if (joined) p = sum_of_cluster(p, b2, tid, part, g.per_row, ctas);
         soft = Softmax::of(p);
         if (!WHOLE && part == 0 && tid == 0) g.loss[row] = soft.ref, g.lse_out[row] = soft.sum2;
     }
@@ -878,7 +893,7 @@ __global__ void __launch_bounds__(32 * LIST_WARPS) k_listed(const __grid_constan
         if (weight == 0.0f) return Softmax{};
         if (MODE != GRAD) return Softmax::of(g.loss[row], g.lse_out[row]);
         const float lse = g.lse_in[row], b2 = g.beta * LOG2E;
-        if (!(fabsf(lse) > LSE_KEPT)) return Softmax::of_lse(lse, g.beta);
+        if (!(fabsf(lse) > LSE_KEPT)) return Softmax::of_lse(lse, g.beta, g.per_beta);
         const T* logits = static_cast<const T*>(g.logits) + row * g.pitch;
         return Softmax::of(teams == 1 ? sum_again<T, 32 * LIST_WARPS>(logits, g.cols, b2, me, warps) : sum_again<T, 32>(logits, g.cols, b2, me, warps));
     };
@@ -909,7 +924,10 @@ int32_t launch_distill(thrml_ctx* ctx, cudaStream_t stream, DistillArgs g) {
     // most that have to join; with few rows more, so that the GPU is covered.
     const int64_t span = positions<T>(g.logits, g.pitch, g.cols), held = (MODE == LOSS ? 4 : 1) * SOFTMAX_BYTES / sizeof(T);
     int64_t per_row = (span + held - 1) / held;
-    if (MODE != GRAD) per_row = std::min<int64_t>(per_row, 8);
+    // A gradient's CTAs work apart, and each forms the sums of a row whose lse it does not take by itself; rows that more than SUMMED_APART
+    // would read so share them as in the other modes.
+    const bool whole_long = MODE == GRAD && per_row > SUMMED_APART;
+    if (MODE != GRAD || whole_long) per_row = std::min<int64_t>(per_row, 8);
     while (per_row <= 4 && g.rows * per_row < 2 * ctx->sm_count && span / (2 * per_row) >= SOFTMAX_THREADS * VEC<T>) per_row *= 2;
     if (g.rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
     g.per_row = static_cast<int32_t>(per_row);
@@ -922,9 +940,10 @@ int32_t launch_distill(thrml_ctx* ctx, cudaStream_t stream, DistillArgs g) {
     cfg.attrs = &attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {static_cast<unsigned>(per_row), 1, 1};
-    cfg.numAttrs = MODE != GRAD && per_row > 1 ? 1 : 0;
+    g.joined = (MODE != GRAD || whole_long) && per_row > 1;
+    cfg.numAttrs = g.joined ? 1 : 0;
     const size_t list_bytes = 4 * static_cast<size_t>(list_words(g.top, MODE));
-    if (g.rows * per_row <= 2 * ctx->sm_count) {
+    if (g.rows * per_row <= 2 * ctx->sm_count || whole_long) {
         cfg.dynamicSmemBytes = list_bytes;
         CU_TRY(cudaLaunchKernelEx(&cfg, k_softmax<T, MODE, true>, g));
         return THRML_OK;
@@ -979,6 +998,7 @@ DistillArgs distill_args(const void* logits, int64_t pitch, int64_t cols, int64_
     g.teacher_type = teacher_type;
     g.teacher_pitch = teacher_pitch;
     g.beta = beta;
+    g.per_beta = 1.0f / beta;
     g.weight = weight;
     return g;
 }
