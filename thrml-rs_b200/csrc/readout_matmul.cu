@@ -384,19 +384,16 @@ __global__ void __launch_bounds__(PROD_THREADS<BM>)
         cluster_sync_all();  // every CTA's sums have arrived
         if (warp >= 2 && !lost.raised()) {
             const int quarter = warp & 3, ch = quarter * 32 + lane;
-            const int32_t col = n0 + ch, share = BM / static_cast<int32_t>(split);
+            const int32_t col = n0 + ch, share = BM / static_cast<int32_t>(split), first = m0 + static_cast<int32_t>(rank) * share;
             const int32_t* red = reinterpret_cast<const int32_t*>(smem + STAGES * STAGE_BYTES);
-            if (col < g.n) {
-                const float w_scale = g.w_scale[col], bias = g.bias ? g.bias[col] : 0.0f;
-                T* out = static_cast<T*>(g.out) + col;
-                for (int32_t t = (warp - 2) >> 2; t < share; t += (PROD_THREADS<BM> - 64) / 128) {
-                    const int32_t token = m0 + static_cast<int32_t>(rank) * share + t;
-                    if (token >= g.m) break;
-                    int32_t acc = 0;
-                    for (uint32_t src = 0; src < split; ++src) acc += red[(src * share + t) * TILE_N + ch];
-                    const float y = __int2float_rn(acc) * a_scale(token) * w_scale;
-                    out[token * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
-                }
+            const float w_scale = col < g.n ? g.w_scale[col] : 0.0f, bias = g.bias && col < g.n ? g.bias[col] : 0.0f;
+            const float held = lane < share && first + lane < g.m ? a_scale(first + lane) : 0.0f;  // a lane for each token: at most 32
+            T* out = static_cast<T*>(g.out) + col;
+            for (int32_t t = (warp - 2) >> 2; t < share && first + t < g.m; t += (PROD_THREADS<BM> - 64) / 128) {
+                int32_t acc = 0;
+                for (uint32_t src = 0; src < split; ++src) acc += red[(src * share + t) * TILE_N + ch];
+                const float y = __int2float_rn(acc) * __shfl_sync(0xffffffffu, held, t) * w_scale;
+                if (col < g.n) out[(first + t) * g.out_pitch] = from_float<T>(g.bias ? y + bias : y);
             }
         }
     }
@@ -456,6 +453,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2], settle_bar;
     __shared__ uint32_t tmem_base_slot;
     __shared__ int lost_word, peer_issued;
+    // Of a warp's half of the tile's tokens: four of them come by one instruction, where each by a load of its own held the epilogue up
+    // behind short sums (8192 x 784 -> 4096: 67 -> 49 us; 58 by read-only loads, which memory that k_quantize may be writing rules out).
+    __shared__ __align__(16) float token_scales[8][BM / 2];
 
     const SharedWord lost{smem_u32(&lost_word)};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -548,6 +548,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2, ch = quarter * 32 + lane;
         uint32_t it = 0;
+        float* mine = token_scales[warp - 2];
         asm volatile("griddepcontrol.wait;" ::: "memory");  // the tokens' scales
         for (int32_t tile = first_tile; tile < args.tiles; tile += tile_step, ++it) {
             int32_t tm, tn;
@@ -555,20 +556,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
             const uint32_t buf = it & 1u;
             const int32_t col = tn * PAIR_CHANNELS + static_cast<int32_t>(rank) * TILE_N + ch, m0 = tm * BM + half * (BM / 2);
             const float w_scale = col < g.n ? g.w_scale[col] : 0.0f, bias = g.bias && col < g.n ? g.bias[col] : 0.0f;
+            __syncwarp();  // the last tile's have been read
+#pragma unroll
+            for (int t = 0; t < BM / 64; ++t) mine[32 * t + lane] = m0 + 32 * t + lane < g.m ? g.a_scale[m0 + 32 * t + lane] : 0.0f;
+            __syncwarp();
             if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (it >> 1) & 1u, lost, 4))) break;  // the lanes go on together
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t taddr = tmem + buf * BM + half * (BM / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
             T* out = static_cast<T*>(g.out) + static_cast<int64_t>(m0) * g.out_pitch + col;
 #pragma unroll 1
             for (int c = 0; c < BM / 32; ++c) {
+                const int32_t left = g.m - (m0 + c * 16);  // tokens from here on
                 uint32_t acc[16];
                 tmem_ld16_issue(taddr + c * 16, acc);
-                tmem_ld_wait();
-                const int32_t left = g.m - (m0 + c * 16);  // tokens from here on
-                if (col < g.n) {
-                    float scales[16];  // by plain loads (see k_product), before the stores
+                float scales[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) scales[j] = j < left ? g.a_scale[m0 + c * 16 + j] : 0.0f;
+                for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(scales + j) = *reinterpret_cast<const float4*>(mine + c * 16 + j);
+                tmem_ld_wait();
+                if (col < g.n) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (j < left) {
