@@ -541,8 +541,8 @@ int32_t thrml_ctx_reset_waits(thrml_ctx* ctx);
 int32_t thrml_quantize_rows_i8(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* x, int32_t x_type, int64_t x_pitch, int8_t* q, int64_t q_pitch,
                                float* scale);
 /* out[i][j] = (sum_k a[i][k] w[j][k]) * a_scale[i] * w_scale[j] + bias[j] (bias f32, nullable): 8-bit integers, one scale for
- * each token (row of a) and channel (row of w), the sum exact in 32-bit integers (k at most 131071), the rest in f32, rounded
- * once to out_type.  a and w start on 16-byte boundaries and their pitches are multiples of 16. */
+ * each token (row of a) and channel (row of w), the sum exact in 32-bit integers (k at most 131071), the rest in f32 (the sum's
+ * conversion, each scale and the bias round once), then rounded to out_type.  a and w start on 16-byte boundaries and their pitches are multiples of 16. */
 int32_t thrml_matmul_i8(thrml_ctx* ctx, void* stream, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_pitch, const float* a_scale, const int8_t* w,
                         int64_t w_pitch, const float* w_scale, const float* bias, void* out, int32_t out_type, int64_t out_pitch);
 /* Both: x is quantised, then multiplied.  q (16-byte boundary, pitch a multiple of 16) and scale are the caller's workspaces; what
@@ -581,7 +581,9 @@ int32_t thrml_adjust_logits(thrml_ctx* ctx, void* stream, int64_t rows, int64_t 
  * or whose beta is negative or NaN, gets -1.  The uniforms: noise[r][k] in (0, 1) (f32, device; the injected noise of a
  * parity run), or with noise NULL the 23-bit uniform of word k & 3 of Philox4x32-10(counter (row_offset + r, 0, k >> 2, 'DRAW'), key),
  * so that results do not depend on how rows are sharded (row_offset + rows <= 2^32).  Scores that lie near the largest
- * are compared in f64. */
+ * are compared in f64.  A captured call keeps its key: its replays draw with the same noise.  23 bits resolve chances to a fraction of cols
+ * 2^-23 (equal logits: the first of 131072 is drawn 1.6 % more often than the last), and a category whose beta * logit lies 19.5 or
+ * more below the largest is never drawn. */
 int32_t thrml_draw_categories(thrml_ctx* ctx, void* stream, int64_t rows, int64_t cols, const void* logits, int32_t type, int64_t pitch, const float* beta, uint64_t key,
                               int64_t row_offset, const float* noise, int64_t noise_pitch, int64_t* out);
 /* Distillation from a teacher's top logits.  Row r lists categories ids[r][0 .. top) (top <= 1024; THRML_I32 or THRML_I64) with the teacher's logits;

@@ -45,7 +45,8 @@ __device__ __forceinline__ uint4 nothing_16() {
 // in flight together; meanwhile it counts there those of the row's tokens that fall into the share (integer atomics, so the counts
 // do not depend on their order).  A count has 16 bits, and 32 in rows of 2^15 tokens or more (and where the repetition penalty has no reciprocal in f32), which are done half a share at a time.
 // Every CTA of a row reads the whole history, from L2 after the first.  256 x 131072 bf16 with 4096 tokens, biases and masks 56 us =
-// 2.4 TB/s, bound by instruction issue; without any rule 23, by memory.
+// 2.4 TB/s: issue slots are busy for 69 % of it (39 M warp instructions, 35 us at full issue), shared memory and barriers hold the rest;
+// without any rule 23, by memory.
 // Categories with a bias are finished by a thread of their own, before the pass over the share, which leaves out what a bitmap
 // marks.  Measured and dropped for 256 rows of 131072 bf16 with 3000 tokens each: the few named categories in a kernel of
 // their own behind a plain copy, 77 us (their scattered 2-byte writes cost more than they are); for 16 rows with 60000
@@ -276,7 +277,8 @@ __global__ void __launch_bounds__(ADJUST_THREADS, 3) k_adjust(const __grid_const
 // hardware exponential and no logarithm, and nearly every category fails it.  The ones that pass get their score in f64
 // (where two scores that f32 cannot tell apart have an order), which decides.  B starts from approximate scores of each
 // thread's first categories, lowered by more than their error, and rises with the scores found, shared in the CTA.
-// Bound by instruction issue: ten rounds of the generator serve four categories.  256 x 131072 bf16: 52 us with two CTAs a
+// Ten dependent rounds of the generator serve four categories: half of 23 M warp instructions for 256 x 131072 bf16, 20 us at full
+// issue, of which they reach 49 % (waits for memory, for the rounds' results and at barriers hold the rest): 52 us with two CTAs a
 // row, 60 with four and 75 with eight, whose starts and first, loose bounds cost more than they spread.  Four CTAs of 128
 // threads, which spread evenly over the SMs: 56; 512 x 32000 38 instead of 33, though 2048 x 5003 34 instead of 40.
 // ---------------------------------------------------------------------------------------------------------
@@ -797,7 +799,7 @@ __device__ __forceinline__ void finish_list(const DistillArgs& g, int64_t row, f
 
 // The rows' sums (reference into loss, log2 of the sum into lse_out, from where k_listed takes them), and weight * beta * q into
 // grad.  WHOLE: with few rows the list too, each CTA its own share's (a launch less: a step of 33 x 5003, 20 listed, 17.7 -> 14.6 us as
-// the host sees it, though 6.4 -> 7.0 on the GPU; 33 x 131072, 1024 listed, a gradient 42 -> 12 us).
+// the host sees it, which the choice is made for, though 6.4 -> 7.0 on the GPU, as in a replayed graph; 33 x 131072, 1024 listed, a gradient 42 -> 12 us).
 template <class T, int MODE, bool WHOLE>
 __global__ void __launch_bounds__(SOFTMAX_THREADS, 4) k_softmax(const __grid_constant__ DistillArgs g) {
     constexpr int V = VEC<T>, AT_ONCE = 4;

@@ -32,8 +32,8 @@ __device__ __forceinline__ int32_t quantise(float x, float scale, float inverse)
 
 // Bound by memory.  A CTA has a row: as many threads as hold it in two 16-byte pieces each (32 to 512; a longer row's rest is
 // read a second time), in registers between the maximum and the quotients.  Four pieces and 256 threads are no faster on rows of 4096
-// (2048 of them, bf16: 11 us against 10.5) and slower on long ones (256 of 131072: 53 against 32); 1024 threads 2048 of 16384: 53
-// against 34.
+// (2048 of them, bf16: 11 us against 10.5) and slower on long ones (256 of 131072: 53 against 32, with all of it in L2; 44 from memory);
+// 1024 threads 2048 of 16384: 53 against 34.
 constexpr int QUANT_THREADS = 512, QUANT_PIECES = 2;
 
 // A row's scale, from the largest magnitude in it.
@@ -160,8 +160,9 @@ constexpr size_t prod_smem(int split) {
 }
 
 // Few tokens of few inputs are quantised by the product's own CTAs (X: their type), each for its part of K: a row's maximum takes
-// the whole row, which every CTA reads, 16 KB in all at most.  That saves a launch: a call with one token, 4096 inputs and
-// channels takes the host 11.7 us instead of 14.3, and the GPU 9.7 instead of 9.0.
+// the whole row, which every CTA reads: 32 KB of f32 in all at most, 16 KB of the 2-byte types.  That saves a launch, and is chosen for
+// that: a call with one token, 4096 inputs and channels takes the host 11.7 us instead of 14.3, but the GPU 9.7 instead of 9.0, which
+// is what a replayed graph of such calls pays.
 constexpr int FEW_VALUES = 8192, FEW_STEPS = 16;  // values of x; steps of K per CTA, whose tokens are held at once
 struct FewTokens {
     const void* x;
@@ -733,7 +734,7 @@ int split_of(const thrml_ctx* ctx, int64_t tiles, int64_t k_steps) {
 template <class T>
 int32_t product(thrml_ctx* ctx, cudaStream_t stream, const Product& p) {
     // Up to 64 tokens, and up to a wave of two CTAs an SM, the operands' way from memory binds, and many CTAs keep more of them
-    // in flight (4096 inputs, 65536 channels: 16 tokens 47 us, in pairs 58; 64 tokens 53, in pairs 61; 4096 channels: 128 tokens
+    // in flight (4096 inputs, 65536 channels: 16 tokens 47 us, in pairs 58; 64 tokens 51, in pairs 61; 4096 channels: 128 tokens
     // 15, in pairs 20; 512 tokens 19, in pairs 22).  Beyond, pairs: with 256 tokens a tile unless 128 need fewer rounds for the
     // half of the work each.
     const int bm = p.m <= 16 ? 16 : p.m <= 32 ? 32 : 64;

@@ -142,7 +142,7 @@ def _int8_rows(x, name, index, cols=None):
 def int8_matmul(q, q_scale, weight, weight_scale, bias=None, out_dtype=None, out=None):
     """(q @ weight.T) * q_scale[:, None] * weight_scale + bias: 8-bit rows `q [tokens, inputs]` and `weight [channels, inputs]`
     (int8, rows on 16-byte boundaries: see `align_rows_int8`), one f32 scale per token and channel, f32 bias.  The sums are
-    exact; the result is rounded once to `out_dtype` (float32, bfloat16 or float16; float32 by default)."""
+    exact; their conversion to f32, the two scales and the bias round once each, and the result to `out_dtype` (float32, bfloat16 or float16; float32 by default)."""
     h, stream, index = _device(q, "q")
     pitch, m, k = _int8_rows(q, "q", index)
     w_pitch, n, _ = _int8_rows(weight, "weight", index, k)
@@ -243,7 +243,10 @@ def draw_categories(logits, key, *, beta=None, row_offset=0, noise=None, out=Non
     gets -1.
 
     key: the seed of an RngKey (or the RngKey); row r's noise depends on the key and on row_offset + r alone, so rows may be
-    sharded.  noise: uniforms in (0, 1) `[rows, categories]` f32 to use instead."""
+    sharded.  A call that is captured into a CUDA graph keeps its key: every replay draws with the same noise (give `noise`, and fill it
+    anew before each).  The key's uniforms are the samplers', of 23 bits: chances follow the softmax to within a fraction of 2^-23 times
+    the number of categories (equal logits among 131072: the first is drawn 1.6 % more often than the last, as ties go to the lowest), and a category
+    whose beta * logit lies 19.5 or more below the largest is never drawn.  noise: uniforms in (0, 1) `[rows, categories]` f32 to use instead."""
     h, stream, index = _device(logits, "logits")
     kind, pitch, rows, cols = _rows(logits, "logits", index)
     u, u_pitch = None, 0
@@ -278,7 +281,8 @@ def distill_loss(logits, ids, teacher, *, beta=1.0, weight=None):
     `ids [rows, top]` (int32 or int64; ids outside the categories, or teacher logits of -inf, are not listed; top <= 1024).
 
     loss[r] = sum_j p_j (log p_j - log q_id(j)) with p = softmax over the listed of beta * teacher and q = softmax of beta * logits;
-    lse = logsumexp(beta * logits), for `distill_grad`.  Rows whose weight is 0 are padding: they are not read and have loss 0."""
+    lse = logsumexp(beta * logits), for `distill_grad`.  Rows whose weight is 0 are padding: they are not read and have loss and lse 0, as
+    rows that list nothing have.  beta is within 2^-100 and 2^100."""
     a, _ = _distill_args(logits, ids, teacher, beta, weight)
     rows = a[2]
     loss = logits.new_empty((2, rows), dtype=torch.float32)
@@ -289,7 +293,7 @@ def distill_loss(logits, ids, teacher, *, beta=1.0, weight=None):
 
 def distill_grad(logits, lse, ids, teacher, *, beta=1.0, weight=None, out=None):
     """The gradient of sum_r weight[r] * loss[r] by the logits, in their type, from `distill_loss`'s lse: weight (f32 per row, None = 1)
-    is what comes from above."""
+    is what comes from above.  An lse beyond +-256 is too coarse to be used: such a row's sums are formed again from its logits."""
     a, index = _distill_args(logits, ids, teacher, beta, weight)
     out, _, pitch = _new_or(out, logits, a[2], a[3], logits.dtype, index)
     if lse is None:
