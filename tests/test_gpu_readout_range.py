@@ -219,9 +219,10 @@ def test_distill_large_logits_with_lists(T, dtype, n, times, top):
         check_large(T, x, ids, torch.randn(5, top, generator=g, device="cuda"), 0.7, times)
 
 
-@pytest.mark.parametrize("dtype, n, rows", [(torch.float32, 1048601, 1), (torch.float32, 1048601, 40), (torch.bfloat16, 4500001, 2), (torch.float16, 2097200, 38)])
+@pytest.mark.parametrize("dtype, n, rows", [(torch.float32, 1048601, 1), (torch.float32, 1048601, 40), (torch.bfloat16, 4500001, 2), (torch.float16, 2097200, 38), (torch.float32, 1048601, 100)])
 def test_distill_rows_beyond_4_mb(T, dtype, n, rows):
-    """A gradient's CTAs share such rows' sums, where they form them again: ordinary rows, a large one among them, one of the lowest value."""
+    """Where sums are formed again, by each of a gradient's CTAs or, for many such rows, shared: ordinary rows, a large one among them, one of
+    the lowest value."""
     x = torch.randn(rows, n, generator=gen(6), device="cuda") * 3
     x[-1] = torch.finfo(dtype).min
     if rows > 1:

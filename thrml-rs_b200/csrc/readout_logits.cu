@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(DRAW_THREADS, 4) k_draw(const __grid_constant_
 constexpr int SOFTMAX_THREADS = 256;
 constexpr int64_t SOFTMAX_BYTES = 64 << 10;  // of a row per CTA
 constexpr int LIST_WARPS = 4;
-constexpr int SUMMED_APART = 64;  // 4 MB of a row
+constexpr int64_t APART_CTAS = 64, APART_BYTES = int64_t{16} << 30;  // see launch_distill
 enum Distill { LOSS, GRAD, STEP };
 
 struct DistillArgs {
@@ -926,9 +926,10 @@ int32_t launch_distill(thrml_ctx* ctx, cudaStream_t stream, DistillArgs g) {
     // most that have to join; with few rows more, so that the GPU is covered.
     const int64_t span = positions<T>(g.logits, g.pitch, g.cols), held = (MODE == LOSS ? 4 : 1) * SOFTMAX_BYTES / sizeof(T);
     int64_t per_row = (span + held - 1) / held;
-    // A gradient's CTAs work apart, and each forms the sums of a row whose lse it does not take by itself; rows that more than SUMMED_APART
-    // would read so share them as in the other modes.
-    const bool whole_long = MODE == GRAD && per_row > SUMMED_APART;
+    // A gradient's CTAs work apart, and each forms the sums of a row whose lse it does not take by itself.  Where that would be more than
+    // APART_BYTES (6 ms) of reading for rows of more than APART_CTAS, they share the sums as in the other modes, by eight CTAs a row at
+    // most.  f32, us a gradient, lse taken / not taken: a row of 8 million, apart, 15 / 5600; ten of them, shared, 228 / 380 (apart 106 / 56000).
+    const bool whole_long = MODE == GRAD && per_row > APART_CTAS && g.rows * per_row > APART_BYTES / (span * static_cast<int64_t>(sizeof(T)));
     if (MODE != GRAD || whole_long) per_row = std::min<int64_t>(per_row, 8);
     while (per_row <= 4 && g.rows * per_row < 2 * ctx->sm_count && span / (2 * per_row) >= SOFTMAX_THREADS * VEC<T>) per_row *= 2;
     if (g.rows * per_row > INT32_MAX) return fail(THRML_ERR_INVALID_ARG, "too many rows of this length in one call");
